@@ -36,6 +36,7 @@ extern "C" {
 #define PGV_ACT_NONE 0
 #define PGV_ACT_LEAKY_RELU 1 /* nn.LeakyReLU(slope)  encoder.py:239-240, decoder.py:203-204 */
 #define PGV_ACT_HARDTANH 2   /* nn.Hardtanh(-1,1)    decoder.py:98,219 */
+#define PGV_ACT_SILU 3       /* x / (1 + exp(-x)); pgv_group_norm_act_* only */
 
 typedef struct pgv_conv_desc {
   int32_t B;               /* batch */
@@ -515,6 +516,71 @@ int pgv_params_loss(const float* u_out, const float* u_in, int B, int L, const p
 int pgv_params_columns(const float* u_out, const float* u_in, int B, int L, int n_items, const int32_t* kind,
                        const int32_t* first, const int32_t* len, const float* card, const int32_t* idx, float* in_cols,
                        float* out_cols, float* match, void* stream);
+
+/* ---- 8-bit operands with one scale per block of 128 -------------------------------------------------- */
+/* (beside pgv_gemm / the weight shadows: the operands of nn.Linear products, model/encoder.py:85, decoder.py:64, held in OCP
+ * 8-bit floating point.)  A matrix [R][C] quantised along its columns is bytes q[R][Kp], Kp = C rounded up to whole blocks of
+ * 128 with zeros behind C, and fp32 scales:
+ *   PGV_F8_ROWS   one per 128 neighbours of a row:  scale[Kp/128][R]
+ *   PGV_F8_TILES  one per 128 x 128 tile:           scale[ceil(R/128)][Kp/128]
+ * amax = max(max |x|, 2^-100) of the block, scale = amax / F, inv = F / amax (both correctly rounded; F = 448 / 57344),
+ * byte = x * inv (one fp32 product) rounded to nearest even.  A block that holds a NaN or an infinity gets scale = NaN and
+ * NaN bytes, so every product that reads it is NaN.  These entry points take fp32, bfloat16 or float16 values (PGV_DT_*). */
+#define PGV_DT_F32 0
+#define PGV_DT_BF16 1
+#define PGV_DT_F16 2
+#define PGV_F8_E4M3 0
+#define PGV_F8_E5M2 1
+#define PGV_F8_ROWS 0
+#define PGV_F8_TILES 1
+#define PGV_F8_BLOCK 128
+#define PGV_F8_MAX_EXTENT (1 << 24) /* rows / columns of a matrix */
+#define PGV_F8_MAX_K (1 << 23)      /* reduction of a product: a tile's rows are addressed with 32 bits */
+/* x[rows][cols] (row stride ldx values) -> q / scale (blocks along cols) and / or qt / scale_t (the same of the transpose:
+ * qt[cols][ceil(rows/128)*128]), either pair nullable; colsum[cols] (nullable) = the fp32 column sums, e.g. a bias gradient
+ * (workspace: pgv_f8_quantize_workspace bytes, needed with colsum only).  x is read once.  q / qt 16-byte aligned. */
+int64_t pgv_f8_quantize_workspace(int64_t rows, int64_t cols);
+int pgv_f8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int block, int fmt, void* q,
+                    float* scale, void* qt, float* scale_t, float* colsum, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+/* out[M][N] = sum_b a_scale[b][m] b_scale[..][b] sum_{k in b} a[m][k] b[n][k] (+ bias[n]), accumulated in fp32, rounded once
+ * to out_dtype.  a: PGV_F8_ROWS of an [M][K] matrix in either format; b: PGV_F8_ROWS or PGV_F8_TILES (b_block) of an [N][K]
+ * matrix in e4m3.  a, b, out 16-byte aligned.  workspace: pgv_f8_matmul_workspace bytes (a reduction split over workgroups
+ * leaves its partial results there; they are added in a fixed order).  Results do not depend on the run. */
+int64_t pgv_f8_matmul_workspace(int64_t M, int64_t N, int64_t K, int b_block);
+int pgv_f8_matmul(int64_t M, int64_t N, int64_t K, const void* a, const float* a_scale, int a_fmt, const void* b,
+                  const float* b_scale, int b_block, const float* bias, void* out, int out_dtype, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+/* nn.Linear on a quantised weight: pgv_f8_quantize (PGV_F8_ROWS, e4m3) of x[M][K], then pgv_f8_matmul; same values.  Where
+ * pgv_f8_linear_fused(M, b_block) is 1 the rows are quantised inside the product and xq / x_scale (bytes [M][Kp] and
+ * [Kp/128][M] otherwise) are not used.  workspace as pgv_f8_matmul. */
+int pgv_f8_linear_fused(int64_t M, int b_block);
+int pgv_f8_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* b, const float* b_scale,
+                  int b_block, int64_t N, const float* bias, void* xq, float* x_scale, void* out, int out_dtype,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- GroupNorm + activation, channels last ------------------------------------------------------------ */
+/* (beside the BatchNorm of the conv blocks, model/layer.py:10-46, for layers whose batch is too small or too ragged for batch
+ * statistics.)  x[N][P][C], values of an item's P pixels with the channels innermost, G groups of C/G channels:
+ *   mean, var (biased) over the P * C/G values of (item, group);  y = act(gamma (x - mean) / sqrt(var + eps) + beta)
+ * gamma / beta [C] fp32, nullable (1 / 0); act: PGV_ACT_* including PGV_ACT_SILU; mean / rstd [N][G] fp32 are outputs of the
+ * forward call and inputs of the backward call.  Statistics and sums in fp32 or fp64, one rounding to dtype at the end.
+ * A pixel that holds a NaN or an infinity makes its (item, group) NaN and no other.
+ * pgv_group_norm_act_f8 writes the result as the PGV_F8_ROWS operand (N * P rows, blocks along the channels) of a product,
+ * quantised from the fp32 values.  workspace: pgv_group_norm_workspace bytes, kind 0 = fwd, 1 = f8, 2 = bwd; 8-byte aligned.
+ * Results do not depend on the run. */
+int64_t pgv_group_norm_workspace(int64_t N, int64_t P, int64_t C, int64_t G, int dtype, int kind);
+int pgv_group_norm_act_fwd(const void* x, int dtype, int64_t N, int64_t P, int64_t C, int64_t G, const float* gamma,
+                           const float* beta, float eps, int act, float slope, void* y, float* mean, float* rstd,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+int pgv_group_norm_act_f8(const void* x, int dtype, int64_t N, int64_t P, int64_t C, int64_t G, const float* gamma,
+                          const float* beta, float eps, int act, float slope, int fmt, void* q, float* scale,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+/* ggamma / gbeta [C] fp32, nullable, overwritten. */
+int pgv_group_norm_act_bwd(const void* gy, const void* x, int dtype, int64_t N, int64_t P, int64_t C, int64_t G,
+                           const float* gamma, const float* beta, const float* mean, const float* rstd, int act,
+                           float slope, void* gx, float* ggamma, float* gbeta, void* workspace, int64_t workspace_bytes,
+                           void* stream);
 
 /* ---- misc -------------------------------------------------------------------------------------------- */
 int pgv_fill(float* p, int64_t n, float v, void* stream);

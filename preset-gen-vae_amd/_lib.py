@@ -11,7 +11,7 @@ from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int6
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libpgv_hip.so")
 
-PGV_ACT_NONE, PGV_ACT_LEAKY_RELU, PGV_ACT_HARDTANH = 0, 1, 2
+PGV_ACT_NONE, PGV_ACT_LEAKY_RELU, PGV_ACT_HARDTANH, PGV_ACT_SILU = 0, 1, 2, 3
 PGV_PREZEROED = 1
 
 
@@ -151,6 +151,20 @@ SIGNATURES = {
     "pgv_fill": (c_int, [_P, c_int64, c_float, _P]),
     "pgv_params_loss": (c_int, [_P, _P, c_int, c_int, _PT, c_int, c_float, c_int, c_float, _P, _P, _P, c_int64, _P]),
     "pgv_params_columns": (c_int, [_P, _P, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "pgv_f8_quantize_workspace": (c_int64, [c_int64, c_int64]),
+    "pgv_f8_quantize": (c_int, [_P, c_int, c_int64, c_int64, c_int64, c_int, c_int, _P, _P, _P, _P, _P, _P, c_int64, _P]),
+    "pgv_f8_matmul_workspace": (c_int64, [c_int64, c_int64, c_int64, c_int]),
+    "pgv_f8_matmul": (c_int, [c_int64, c_int64, c_int64, _P, _P, c_int, _P, _P, c_int, _P, _P, c_int, _P, c_int64, _P]),
+    "pgv_f8_linear_fused": (c_int, [c_int64, c_int]),
+    "pgv_f8_linear": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, _P, c_int, c_int64, _P, _P, _P, _P, c_int, _P,
+                              c_int64, _P]),
+    "pgv_group_norm_workspace": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int, c_int]),
+    "pgv_group_norm_act_fwd": (c_int, [_P, c_int, c_int64, c_int64, c_int64, c_int64, _P, _P, c_float, c_int, c_float, _P, _P, _P,
+                                       _P, c_int64, _P]),
+    "pgv_group_norm_act_f8": (c_int, [_P, c_int, c_int64, c_int64, c_int64, c_int64, _P, _P, c_float, c_int, c_float, c_int, _P,
+                                      _P, _P, c_int64, _P]),
+    "pgv_group_norm_act_bwd": (c_int, [_P, _P, c_int, c_int64, c_int64, c_int64, c_int64, _P, _P, _P, _P, c_int, c_float, _P, _P,
+                                       _P, _P, c_int64, _P]),
     "pgv_axpy": (c_int, [c_int64, c_float, _P, _P, _P]),
     "pgv_copy": (c_int, [_P, _P, c_int64, _P]),
     "pgv_probe_mfma": (c_int, [c_int, c_int, _P, POINTER(c_int64), _P]),

@@ -11,7 +11,10 @@ OUT = os.path.join(HERE, "libpgv_hip.so")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-Wno-unused-result"]
 # per-file extras: the FFT butterflies are complex arithmetic on register pairs - packing them into v_pk_* instructions
 # (SLP vectoriser) costs more register moves than it saves: 1560 -> 1376 instructions per frame pair without it
-EXTRA = {"stft_mel.hip": ["-fno-slp-vectorize"]}
+# the 8-bit operand and group-norm kernels: without the packed fp32 instructions
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+EXTRA = {"stft_mel.hip": ["-fno-slp-vectorize"], "f8_quant.hip": NO_PACKED_FP32, "f8_gemm.hip": NO_PACKED_FP32,
+         "group_norm.hip": NO_PACKED_FP32}
 
 
 def sources():

@@ -17,7 +17,8 @@ model.run_name = '00_debug'                    # config.py:21
 model.logs_root_dir = "saved"                  # config.py:75
 model.increased_dataset_size = None            # config.py:41, see update_dynamic_config_params()
 model.encoder_architecture = 'speccnn8l1_bn'   # config.py:24 ; 'speccnn4l1_bn' = BASELINE "4-layer conv-VAE"
-model.params_regression_architecture = 'mlp_3l1024'   # config.py:26 (flow_* variants are out of scope)
+model.params_regression_architecture = 'mlp_3l1024'   # config.py:26 (flow_* variants are out of scope);
+#   not reference values: 'mlp_3l1024_fp8' / '_gn' / '_gn_fp8' (8-bit Linear products, GroupNorm; model/regression.py)
 model.params_reg_softmax = False               # config.py:27
 model.note_duration = (3.0, 1.0)               # config.py:29
 model.sampling_rate = 22050                    # config.py:30

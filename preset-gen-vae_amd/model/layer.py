@@ -783,3 +783,165 @@ class BatchNorm1dFn(torch.autograd.Function):
         x3, g3 = x.view(B, C, 1), g.view(B, C, 1)
         ops.act_bn_bwd(g3, x3, scale, None, None, None, PGV_ACT_NONE, 0.0, gx.view(B, C, 1), None)
         return gx, None, None, None, None
+
+
+# ---- 8-bit Linear and channels-last GroupNorm ---------------------------------------------------------------------------
+def _clean_grad_view(param):
+    """The flat-buffer gradient slice of ``param`` if it still holds this step's zeros (a kernel may then store into it),
+    else None: the gradient goes back to autograd, which adds it to whatever the slice holds - a layer applied twice, a
+    second backward without ``zero_grad()``."""
+    if param is None or getattr(param, '_pgv_grad_view', None) is None or getattr(param, '_pgv_shared', False):
+        return None
+    view, _, clean = _grad_dest(param, accumulated=True)
+    return view if clean else None
+
+
+class Fp8LinearFn(torch.autograd.Function):
+    """nn.Linear with both operands of its three products in block-scaled 8-bit floating point (``ops.fp8_linear_fwd`` /
+    ``ops.fp8_linear_bwd``): x [M, K] and w [N, K] float32 / bfloat16 / float16, y in the type of x, gradients in the types of
+    their tensors.  Saved for backward: the 8-bit operands, not the values.  Like every function here it is captured into a
+    graph together with its forward pass, with no eager graph of the same parameters alive (VAETrainStep's order: warm up on a
+    side stream, drop the results, capture)."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, grad_fmt='e4m3'):
+        y, saved = ops.fp8_linear_fwd(x, w, None if b is None else b.float())
+        ctx.save_for_backward(saved.xt.q, saved.xt.scale, saved.wt.q, saved.wt.scale)
+        ctx.meta = (saved.xt.cols, saved.wt.cols, x.dtype, w.dtype, b is not None, grad_fmt)
+        ctx.params = (w, b)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        xq, xs, wq, ws = ctx.saved_tensors
+        M, N, x_dtype, w_dtype, has_bias, grad_fmt = ctx.meta
+        w, b = ctx.params
+        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], has_bias and ctx.needs_input_grad[2])
+        saved = ops.Fp8LinearSaved(ops.Fp8Blocks(xq, xs, 'row', M), ops.Fp8Blocks(wq, ws, 'tile', N), x_dtype, w_dtype, has_bias)
+        gw_view = _clean_grad_view(w) if need[1] else None
+        gb_view = _clean_grad_view(b) if need[2] else None
+        gx, gw, gb = ops.fp8_linear_bwd(gy.contiguous(), saved, grad_fmt, need, gw_out=gw_view, gb_out=gb_view)
+        if gw_view is not None or gb_view is not None:
+            _grad_done(w if gw_view is not None else None, b if gb_view is not None else None)
+        if gb is not None and gb_view is None:
+            gb = gb.to(b.dtype)
+        return gx, None if gw_view is not None else gw, None if gb_view is not None else gb, None
+
+
+class Fp8Linear(nn.Linear):
+    """``nn.Linear`` (same parameters and state-dict keys) whose products run on 8-bit operands with one scale per block of
+    128: activations per row, weights per 128 x 128 tile.  ``grad_fmt``: the 8-bit format of the output gradient ('e4m3', or
+    'e5m2' for its wider range).
+
+    Serving: ``quantize_weight()`` lays the weight out once (1 byte per value); until the next ``train()``, device move or
+    ``load_state_dict`` calls without gradients use it instead of the master weight."""
+
+    def __init__(self, in_features, out_features, bias=True, device=None, dtype=None, grad_fmt='e4m3'):
+        super().__init__(in_features, out_features, bias, device, dtype)
+        if grad_fmt not in ops.F8_FORMATS:
+            raise ValueError(f"grad_fmt is 'e4m3' or 'e5m2', got {grad_fmt!r}")
+        self.grad_fmt = grad_fmt
+        self._weight8 = None
+
+    def quantize_weight(self):
+        self._weight8 = ops.fp8_quantize(self.weight.detach(), 'tile')
+        return self
+
+    def train(self, mode=True):
+        if mode:
+            self._weight8 = None
+        return super().train(mode)
+
+    def _apply(self, fn, *args, **kwargs):
+        self._weight8 = None
+        return super()._apply(fn, *args, **kwargs)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._weight8 = None
+        return super()._load_from_state_dict(*args, **kwargs)
+
+    def forward(self, x):
+        x2 = x.reshape(-1, self.in_features)
+        if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad or
+                                        (self.bias is not None and self.bias.requires_grad)):
+            y = Fp8LinearFn.apply(x2, self.weight, self.bias, self.grad_fmt)
+        else:
+            w8 = self._weight8 if self._weight8 is not None else ops.fp8_quantize(self.weight.detach(), 'tile')
+            y = ops.fp8_linear(x2, w8, None if self.bias is None else self.bias.detach().float())
+        return y.view(*x.shape[:-1], self.out_features)
+
+
+def _norm_act_code(activation):
+    """Activations of ``GroupNormAct``: those of the conv epilogues and SiLU."""
+    return (ops.PGV_ACT_SILU, 0.0) if isinstance(activation, nn.SiLU) else _act_code(activation)
+
+
+class GroupNormActFn(torch.autograd.Function):
+    """GroupNorm + activation over x [items, pixels, channels] (``ops.group_norm_act_fwd`` / ``_bwd``)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act, slope):
+        f32 = [None if t is None else t.detach().float() for t in (weight, bias)]
+        y, mean, rstd = ops.group_norm_act_fwd(x, groups, f32[0], f32[1], eps, act, slope)
+        ctx.save_for_backward(x, mean, rstd, *(t for t in f32 if t is not None))
+        ctx.meta = (groups, act, slope)
+        ctx.params = (weight, bias)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, mean, rstd, *f32 = ctx.saved_tensors
+        weight, bias = ctx.params
+        wf = f32.pop(0) if weight is not None else None
+        bf = f32.pop(0) if bias is not None else None
+        groups, act, slope = ctx.meta
+        need_w = weight is not None and ctx.needs_input_grad[1]
+        need_b = bias is not None and ctx.needs_input_grad[2]
+        gw_view = _clean_grad_view(weight) if need_w else None
+        gb_view = _clean_grad_view(bias) if need_b else None
+        gx, gw, gb = ops.group_norm_act_bwd(gy.contiguous(), x, mean, rstd, groups, wf, bf, act, slope,
+                                            need_params=need_w or need_b, ggamma=gw_view, gbeta=gb_view)
+        if gw_view is not None or gb_view is not None:
+            _grad_done(weight if gw_view is not None else None, bias if gb_view is not None else None)
+        gw = gw.to(weight.dtype) if need_w and gw_view is None else None
+        gb = gb.to(bias.dtype) if need_b and gb_view is None else None
+        return gx if ctx.needs_input_grad[0] else None, gw, gb, None, None, None, None
+
+
+class GroupNormAct(nn.Module):
+    """GroupNorm followed by an activation (LeakyReLU, ReLU, Hardtanh(-1, 1), SiLU or None) in one kernel pass, for tensors [N, C]
+    or [N, C, ...] kept channels last (``memory_format=torch.channels_last``; anything else is brought into that order first,
+    and the output has it).  Parameter names as ``nn.GroupNorm``."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, activation=None, device=None, dtype=None):
+        super().__init__()
+        if num_groups < 1 or num_channels % num_groups:
+            raise ValueError(f"{num_channels} channels do not divide into {num_groups} groups")
+        self.num_groups, self.num_channels, self.eps, self.affine = num_groups, num_channels, eps, affine
+        self.act, self.slope = _norm_act_code(activation)
+        for name, fill in (('weight', torch.ones), ('bias', torch.zeros)):
+            self.register_parameter(name, nn.Parameter(fill(num_channels, device=device, dtype=dtype)) if affine else None)
+
+    def extra_repr(self):
+        return f"{self.num_groups}, {self.num_channels}, eps={self.eps}, affine={self.affine}"
+
+    def _rows(self, x):
+        if x.dim() < 2 or x.shape[1] != self.num_channels:
+            raise ValueError(f"expected [N, {self.num_channels}, ...], got {tuple(x.shape)}")
+        pixels = 1
+        for v in x.shape[2:]:
+            pixels *= v
+        return x.movedim(1, -1).contiguous().view(x.shape[0], pixels, self.num_channels)
+
+    def forward(self, x):
+        y = GroupNormActFn.apply(self._rows(x), self.weight, self.bias, self.num_groups, self.eps, self.act, self.slope)
+        return y.view(x.shape[0], *x.shape[2:], self.num_channels).movedim(-1, 1)
+
+    @torch.no_grad()
+    def forward_fp8(self, x, fmt='e4m3'):
+        """The result as the quantised operand of a pointwise product: ``ops.Fp8Blocks`` of the [N * pixels, C] matrix (no
+        gradients)."""
+        w, b = (None if t is None else t.detach().float() for t in (self.weight, self.bias))
+        return ops.group_norm_act_fp8(self._rows(x.detach()), self.num_groups, w, b, self.eps, self.act, self.slope, fmt)

@@ -4,8 +4,14 @@ SURVEY.md §8 row a14 keeps this network only as a *parity output* ("preset-regr
 are <1 % of the step and stock rocBLAS GEMMs through torch are explicitly acceptable there, so ``MLPRegression`` is
 built from stock ``torch.nn`` modules with the reference's sub-module names (``reg_model.fc1``, ``bn1``, ``drp1``,
 ``act1`` ... ``fcN``, ``act``; reference regression.py:61-102).  ``FlowRegression`` (nflows) is out of scope.
+
+Two architecture suffixes run it on the HIP kernels instead (``mlp_3l1024_fp8``, ``mlp_3l1024_gn``, ``mlp_3l1024_gn_fp8``):
+``fp8`` takes ``layer.Fp8Linear`` for every Linear (same parameters), ``gn`` a per-item GroupNorm with the ReLU in the same pass
+(``gnN`` in place of ``bnN`` and ``actN``) where the batch is too small for batch statistics.
 """
 import torch.nn as nn
+
+from . import layer
 
 
 class PresetActivation(nn.Module):
@@ -40,17 +46,24 @@ class MLPRegression(nn.Module):
         self.architecture = architecture.split('_')
         self.dim_z = dim_z
         self.idx_helper = idx_helper
-        if len(self.architecture) != 1:
-            raise NotImplementedError("Arch suffix arguments not implemented yet")
+        suffixes = set(self.architecture[1:])
+        if suffixes - {'fp8', 'gn'} or len(suffixes) != len(self.architecture) - 1:
+            raise NotImplementedError(f"Arch suffix arguments {sorted(self.architecture[1:])} not implemented (fp8, gn)")
+        linear = layer.Fp8Linear if 'fp8' in suffixes else nn.Linear
         n_layers, n_neurons = (int(v) for v in self.architecture[0].split('l'))
         self.reg_model = nn.Sequential()
         for l in range(n_layers):
-            self.reg_model.add_module('fc{}'.format(l + 1), nn.Linear(dim_z if l == 0 else n_neurons, n_neurons))
+            self.reg_model.add_module('fc{}'.format(l + 1), linear(dim_z if l == 0 else n_neurons, n_neurons))
+            if l < n_layers - 1 and 'gn' in suffixes:
+                groups = n_neurons // 32 if n_neurons % 32 == 0 else 1
+                self.reg_model.add_module('gn{}'.format(l + 1), layer.GroupNormAct(groups, n_neurons, activation=nn.ReLU()))
+                self.reg_model.add_module('drp{}'.format(l + 1), nn.Dropout(dropout_p))
+                continue
             if l < n_layers - 1:  # no BN / dropout in the two last FC layers (regression.py:89-93)
                 self.reg_model.add_module('bn{}'.format(l + 1), nn.BatchNorm1d(num_features=n_neurons))
                 self.reg_model.add_module('drp{}'.format(l + 1), nn.Dropout(dropout_p))
             self.reg_model.add_module('act{}'.format(l + 1), nn.ReLU())
-        self.reg_model.add_module('fc{}'.format(n_layers + 1), nn.Linear(n_neurons, idx_helper.learnable_preset_size))
+        self.reg_model.add_module('fc{}'.format(n_layers + 1), linear(n_neurons, idx_helper.learnable_preset_size))
         self.reg_model.add_module('act', PresetActivation(idx_helper, cat_softmax_activation=cat_softmax_activation))
 
     def forward(self, z_K):

@@ -2,11 +2,13 @@
 HIP stream, every arithmetic step runs in the hand-written gfx950 kernels.  No wrapper has a CPU path: tensors must
 be fp32, contiguous and on a ROCm device, otherwise a ``RuntimeError`` is raised."""
 import ctypes
+import functools
+from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from ._lib import PGV_ACT_HARDTANH, PGV_ACT_LEAKY_RELU, PGV_ACT_NONE, ConvDesc  # noqa: F401
+from ._lib import PGV_ACT_HARDTANH, PGV_ACT_LEAKY_RELU, PGV_ACT_NONE, PGV_ACT_SILU, ConvDesc  # noqa: F401
 
 
 def _stream():
@@ -872,3 +874,353 @@ def params_columns(u_out, u_in, item_tables, want_cols=True, want_match=True):
                                               _p(idx), _p(in_cols), _p(out_cols), _p(match), _stream()),
                "pgv_params_columns")
     return in_cols, out_cols, match
+
+
+# ---- 8-bit operands with one scale per block of 128 -------------------------------------------------------------------
+# Values come in and results leave as float32, bfloat16 or float16; sums are float32.  Same contract as the other wrappers
+# (ROCm tensors only, current stream of the tensors' device, nothing synchronises), with two additions: a matrix may have a
+# row stride larger than its width, and calls on another device than the current one switch to it.  Buffers are allocated
+# per call, from the pool of the graph being captured when there is one, so two graphs never share scratch.
+F8_FORMATS = {'e4m3': (0, torch.float8_e4m3fn), 'e5m2': (1, torch.float8_e5m2)}
+F8_BLOCK_KINDS = {'row': 0, 'tile': 1}
+_F8_CODE = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
+_DT_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_F8_EMPTY_SCALE = {'row': lambda r, kb: (kb, r), 'tile': lambda r, kb: (-(-r // 128), kb)}
+
+
+class Fp8Blocks(NamedTuple):
+    """A matrix [R, cols] in 8-bit floating point (``pgv_f8_quantize``): ``q`` [R, Kp] (float8_e4m3fn / float8_e5m2, Kp =
+    ``cols`` rounded up to whole blocks of 128, zeros behind ``cols``), ``scale`` (float32) = [Kp/128, R] for ``block`` =
+    'row' (128 neighbours of a row share a scale) or [ceil(R/128), Kp/128] for 'tile' (128 x 128 values do)."""
+    q: torch.Tensor
+    scale: torch.Tensor
+    block: str
+    cols: int
+
+    def dequantize(self):
+        """The float32 values it stands for, [R, cols] (plain torch: a check and export aid, not a fast path)."""
+        R = self.q.shape[0]
+        s = self.scale.t() if self.block == 'row' else self.scale.repeat_interleave(128, 0)[:R]
+        return (self.q.float().view(R, -1, 128) * s.unsqueeze(-1)).view(R, -1)[:, :self.cols]
+
+
+class _on_device:
+    """Makes the device of ``t`` current for a call (a no-op in the usual case) and gives its stream."""
+    __slots__ = ('guard', 'device')
+
+    def __init__(self, t):
+        self.device = t.device
+        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _values(who, t, ndim=2):
+    """(element type code) of a value tensor; raises on anything the kernels do not read."""
+    if not t.is_cuda:
+        raise RuntimeError("preset-gen-vae_amd ops need tensors on a ROCm device (no CPU fallback exists)")
+    code = _DT_CODE.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"{who}: expected float32, bfloat16 or float16 values, got {t.dtype}")
+    if t.dim() != ndim:
+        raise ValueError(f"{who}: expected a {ndim}-d tensor, got shape {tuple(t.shape)}")
+    return code
+
+
+def _row_stride(who, t):
+    """Row stride of a matrix with neighbouring columns (a matrix of one row or column may carry any stride)."""
+    R, C = t.shape
+    if C > 1 and t.stride(1) != 1:
+        raise RuntimeError(f"{who}: the columns of a row must be neighbours in memory")
+    ld = t.stride(0) if R > 1 else C
+    if ld < C:
+        raise RuntimeError(f"{who}: rows overlap (row stride {ld} < {C} columns)")
+    return ld
+
+
+def _same_device(who, t, *others):
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise RuntimeError(f"{who}: tensors on different devices ({t.device} and {o.device})")
+
+
+def _f32_vector(who, name, t, n):
+    if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != n):
+        raise ValueError(f"{who}: {name} must be {n} contiguous float32 values")
+
+
+def _f8_alloc(R, C, block, fmt, device):
+    Kp = (C + 127) // 128 * 128
+    return Fp8Blocks(torch.empty((R, Kp), dtype=F8_FORMATS[fmt][1], device=device),
+                     torch.empty(_F8_EMPTY_SCALE[block](R, Kp // 128), dtype=torch.float32, device=device), block, C)
+
+
+def _f8_quantize(x, block, fmt, want, want_t, colsum=False):
+    if block not in F8_BLOCK_KINDS or fmt not in F8_FORMATS:
+        raise ValueError(f"fp8_quantize: block is 'row' or 'tile', fmt 'e4m3' or 'e5m2' (got {block!r}, {fmt!r})")
+    code = _values("fp8_quantize", x)
+    ld = _row_stride("fp8_quantize", x)
+    R, C = x.shape
+    dev = x.device
+    t = _f8_alloc(R, C, block, fmt, dev) if want else None
+    tt = _f8_alloc(C, R, block, fmt, dev) if want_t else None
+    cs = torch.empty(C, dtype=torch.float32, device=dev) if colsum else None
+    if R == 0 or C == 0:
+        return t, tt, cs.zero_() if colsum else None
+    ws = torch.empty((R + 127) // 128 * C, dtype=torch.float32, device=dev) if colsum else None
+    with _on_device(x) as stream:
+        _lib.check(_lib.load().pgv_f8_quantize(x.data_ptr(), code, R, C, ld, F8_BLOCK_KINDS[block], F8_FORMATS[fmt][0],
+                                               t.q.data_ptr() if want else None, t.scale.data_ptr() if want else None,
+                                               tt.q.data_ptr() if want_t else None, tt.scale.data_ptr() if want_t else None,
+                                               _p(cs), _p(ws), 0 if ws is None else ws.numel() * 4, stream),
+                   "pgv_f8_quantize")
+    return t, tt, cs
+
+
+def fp8_quantize(x, block='row', fmt='e4m3'):
+    """x [R, C] -> ``Fp8Blocks`` of x, blocks along the columns (what a product contracts over)."""
+    return _f8_quantize(x, block, fmt, True, False)[0]
+
+
+def fp8_quantize_both(x, block='row', fmt='e4m3'):
+    """(``Fp8Blocks`` of x, ``Fp8Blocks`` of x^T) with x read once.  'tile': the same bytes and scales, transposed; 'row': the
+    transpose has its own scales, one per 128 neighbours of a column of x."""
+    return _f8_quantize(x, block, fmt, True, True)[:2]
+
+
+def _f8_operand(who, t):
+    if not isinstance(t, Fp8Blocks):
+        raise TypeError(f"{who}: expected Fp8Blocks (fp8_quantize), got {type(t).__name__}")
+    q, s, block, cols = t
+    if not q.is_cuda or q.dtype not in _F8_CODE or q.dim() != 2 or not q.is_contiguous():
+        raise RuntimeError(f"{who}: the bytes must be a contiguous 2-d float8 tensor on a ROCm device")
+    if block not in F8_BLOCK_KINDS:
+        raise ValueError(f"{who}: unknown block kind {block!r}")
+    R, Kp = q.shape
+    if Kp != (cols + 127) // 128 * 128:
+        raise ValueError(f"{who}: {cols} columns take rows of {(cols + 127) // 128 * 128} bytes, got {Kp}")
+    _f32_vector(who, "scale", s, ((R if block == 'row' else (R + 127) // 128) * (Kp // 128)))
+    if tuple(s.shape) != _F8_EMPTY_SCALE[block](R, Kp // 128):
+        raise ValueError(f"{who}: scales of shape {tuple(s.shape)} do not belong to {block} blocks of {tuple(q.shape)}")
+    _same_device(who, q, s)
+    return _F8_CODE[q.dtype]
+
+
+@functools.lru_cache(maxsize=4096)
+def _f8_matmul_ws(M, N, K, b_block):
+    return int(_lib.load().pgv_f8_matmul_workspace(M, N, K, b_block))
+
+
+@functools.lru_cache(maxsize=4096)
+def _f8_fused(M, b_block):
+    return bool(_lib.load().pgv_f8_linear_fused(M, b_block))
+
+
+def _f8_out(who, M, N, dtype, device, out):
+    if dtype not in _DT_CODE:
+        raise ValueError(f"{who}: output type {dtype} is not float32, bfloat16 or float16")
+    if out is None:
+        return torch.empty((M, N), dtype=dtype, device=device)
+    if out.device != device or out.dtype != dtype or tuple(out.shape) != (M, N) or not out.is_contiguous():
+        raise ValueError(f"{who}: out must be a contiguous {dtype} [{M}, {N}] tensor on {device}")
+    return out
+
+
+def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16, out=None):
+    """a [M, K] ('row' blocks, e4m3 or e5m2) times the transpose of b [N, K] ('row' or 'tile' blocks, e4m3), + ``bias`` [N]
+    (float32): [M, N], summed in float32 and rounded once to ``out_dtype`` (``pgv_f8_matmul``)."""
+    fmt = _f8_operand("fp8_matmul", a)
+    if _f8_operand("fp8_matmul", b) != 0:
+        raise ValueError("fp8_matmul: the second operand must be e4m3")
+    if a.block != 'row':
+        raise ValueError("fp8_matmul: the first operand must have 'row' blocks")
+    (M, _), (N, _), K = a.q.shape, b.q.shape, a.cols
+    if b.cols != K:
+        raise ValueError(f"fp8_matmul: reductions of {K} and {b.cols} values")
+    _f32_vector("fp8_matmul", "bias", bias, N)
+    _same_device("fp8_matmul", a.q, b.q, bias)
+    y = _f8_out("fp8_matmul", M, N, out_dtype, a.q.device, out)
+    if M == 0 or N == 0:
+        return y
+    if K == 0:
+        return y.zero_() if bias is None else y.copy_(bias.expand(M, N))
+    kind = F8_BLOCK_KINDS[b.block]
+    nbytes = _f8_matmul_ws(M, N, K, kind)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=y.device) if nbytes else None
+    with _on_device(y) as stream:
+        _lib.check(_lib.load().pgv_f8_matmul(M, N, K, a.q.data_ptr(), a.scale.data_ptr(), fmt, b.q.data_ptr(),
+                                             b.scale.data_ptr(), kind, _p(bias), y.data_ptr(), _DT_CODE[y.dtype], _p(ws),
+                                             nbytes, stream), "pgv_f8_matmul")
+    return y
+
+
+def fp8_linear(x, w, bias=None, out_dtype=None, out=None):
+    """nn.Linear on a weight that was quantised once (``w`` = ``fp8_quantize(weight, 'tile')``): y = Q(x) w^T + bias in the type
+    of x (or ``out_dtype``), Q = 'row' blocks of e4m3 (``pgv_f8_linear``).  Few rows take one launch."""
+    code = _values("fp8_linear", x)
+    ld = _row_stride("fp8_linear", x)
+    if _f8_operand("fp8_linear", w) != 0:
+        raise ValueError("fp8_linear: the weight must be e4m3")
+    (M, K), N = x.shape, w.q.shape[0]
+    if w.cols != K:
+        raise ValueError(f"fp8_linear: x has {K} features, the weight {w.cols}")
+    _f32_vector("fp8_linear", "bias", bias, N)
+    _same_device("fp8_linear", x, w.q, bias)
+    y = _f8_out("fp8_linear", M, N, x.dtype if out_dtype is None else out_dtype, x.device, out)
+    if M == 0 or N == 0:
+        return y
+    if K == 0:
+        return y.zero_() if bias is None else y.copy_(bias.expand(M, N))
+    kind = F8_BLOCK_KINDS[w.block]
+    nbytes = _f8_matmul_ws(M, N, K, kind)
+    xq = None if _f8_fused(M, kind) else _f8_alloc(M, K, 'row', 'e4m3', x.device)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device) if nbytes else None
+    with _on_device(x) as stream:
+        _lib.check(_lib.load().pgv_f8_linear(x.data_ptr(), code, M, K, ld, w.q.data_ptr(), w.scale.data_ptr(), kind, N, _p(bias),
+                                             None if xq is None else xq.q.data_ptr(),
+                                             None if xq is None else xq.scale.data_ptr(), y.data_ptr(), _DT_CODE[y.dtype],
+                                             _p(ws), nbytes, stream), "pgv_f8_linear")
+    return y
+
+
+class Fp8LinearSaved(NamedTuple):
+    """What ``fp8_linear_bwd`` needs from the forward pass: the transposed operands (K + N bytes per row and per weight row
+    instead of the values), the types of x and w."""
+    xt: Fp8Blocks
+    wt: Fp8Blocks
+    x_dtype: torch.dtype
+    w_dtype: torch.dtype
+    has_bias: bool
+
+
+def fp8_linear_fwd(x, w, bias=None):
+    """nn.Linear of a training step: y = Q(x) Q(w)^T + bias in the type of x (x: 'row' blocks, w: 'tile' blocks, both e4m3), and
+    the transposed operands its gradients contract over.  Returns (y, saved)."""
+    if w.dim() != 2 or x.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"fp8_linear_fwd: x {tuple(x.shape)} and w {tuple(w.shape)} do not match")
+    _same_device("fp8_linear_fwd", x, w, bias)
+    x8, xt8 = fp8_quantize_both(x, 'row')
+    w8, wt8 = fp8_quantize_both(w, 'tile')
+    y = fp8_matmul(x8, w8, bias, out_dtype=x.dtype)
+    return y, Fp8LinearSaved(xt8, wt8, x.dtype, w.dtype, bias is not None)
+
+
+def fp8_linear_bwd(gy, saved, grad_fmt='e4m3', need=(True, True, True), gw_out=None, gb_out=None):
+    """Gradients of ``fp8_linear_fwd``: gx = Q(gy) Q(w) in the type of x, gw = Q(gy^T) Q(x^T)^T in the type of w, gb = the
+    column sums of gy in float32 (None without a bias).  ``grad_fmt``: the 8-bit format of gy.  ``need``: which of (gx, gw,
+    gb) are wanted; ``gw_out`` / ``gb_out``: buffers to write instead of new ones.  Returns (gx, gw, gb)."""
+    xt, wt, x_dtype, w_dtype, has_bias = saved
+    (K, _), M, N = xt.q.shape, xt.cols, wt.cols
+    if tuple(gy.shape) != (M, N):
+        raise ValueError(f"fp8_linear_bwd: gy {tuple(gy.shape)}, expected {(M, N)}")
+    _same_device("fp8_linear_bwd", gy, xt.q)
+    need_gb = need[2] and has_bias
+    if not (need[0] or need[1] or need_gb):
+        return None, None, None
+    g8, gt8, gb = _f8_quantize(gy, 'row', grad_fmt, need[0], need[1], colsum=need_gb)
+    if need_gb and gb_out is not None:
+        _f32_vector("fp8_linear_bwd", "gb_out", gb_out, N)
+        gb = gb_out.copy_(gb)
+    gx = fp8_matmul(g8, wt, out_dtype=x_dtype) if need[0] else None
+    gw = fp8_matmul(gt8, xt, out_dtype=w_dtype, out=gw_out) if need[1] else None
+    return gx, gw, gb
+
+
+# ---- GroupNorm + activation, channels last ------------------------------------------------------------------------------
+_GN_FWD, _GN_F8, _GN_BWD = 0, 1, 2
+
+
+@functools.lru_cache(maxsize=4096)
+def _gn_ws(N, P, C, G, code, kind):
+    return int(_lib.load().pgv_group_norm_workspace(N, P, C, G, code, kind))
+
+
+def _gn_args(who, x, groups, weight, bias, act, *others):
+    code = _values(who, x, 3)
+    if not x.is_contiguous():
+        raise RuntimeError(f"{who}: expected a contiguous [items, pixels, channels] tensor")
+    N, P, C = x.shape
+    if groups < 1 or C % groups:
+        raise ValueError(f"{who}: {C} channels do not divide into {groups} groups")
+    if act not in (PGV_ACT_NONE, PGV_ACT_LEAKY_RELU, PGV_ACT_HARDTANH, PGV_ACT_SILU):
+        raise ValueError(f"{who}: unknown activation code {act!r}")
+    _f32_vector(who, "weight", weight, C)
+    _f32_vector(who, "bias", bias, C)
+    _same_device(who, x, weight, bias, *others)
+    return code, N, P, C
+
+
+def group_norm_act_fwd(x, groups, weight=None, bias=None, eps=1e-5, act=PGV_ACT_NONE, slope=0.0):
+    """GroupNorm + activation over x [items, pixels, channels] (contiguous: the memory of an NCHW tensor in channels_last
+    format): (y, mean, rstd), y in the type of x, mean / rstd [items, groups] float32 for ``group_norm_act_bwd``
+    (``pgv_group_norm_act_fwd``).  ``weight`` / ``bias``: float32 [channels] or None."""
+    code, N, P, C = _gn_args("group_norm_act_fwd", x, groups, weight, bias, act)
+    y = torch.empty_like(x)
+    stats = torch.empty((2, N, groups), dtype=torch.float32, device=x.device)
+    mean, rstd = stats[0], stats[1]
+    if x.numel() == 0:
+        if stats.numel():
+            stats.zero_()
+        return y, mean, rstd
+    nbytes = _gn_ws(N, P, C, groups, code, _GN_FWD)
+    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=x.device) if nbytes else None
+    with _on_device(x) as stream:
+        _lib.check(_lib.load().pgv_group_norm_act_fwd(x.data_ptr(), code, N, P, C, groups, _p(weight), _p(bias), eps, act, slope,
+                                                      y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _p(ws), nbytes, stream),
+                   "pgv_group_norm_act_fwd")
+    return y, mean, rstd
+
+
+def group_norm_act_fp8(x, groups, weight=None, bias=None, eps=1e-5, act=PGV_ACT_NONE, slope=0.0, fmt='e4m3'):
+    """``group_norm_act_fwd`` with the result written as the quantised operand of the next product: ``Fp8Blocks`` of the
+    [items * pixels, channels] matrix, 'row' blocks, quantised from the float32 values (``pgv_group_norm_act_f8``)."""
+    code, N, P, C = _gn_args("group_norm_act_fp8", x, groups, weight, bias, act)
+    if fmt not in F8_FORMATS:
+        raise ValueError(f"group_norm_act_fp8: fmt is 'e4m3' or 'e5m2', got {fmt!r}")
+    t = _f8_alloc(N * P, C, 'row', fmt, x.device)
+    if x.numel() == 0:
+        return t
+    nbytes = _gn_ws(N, P, C, groups, code, _GN_F8)
+    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=x.device) if nbytes else None
+    with _on_device(x) as stream:
+        _lib.check(_lib.load().pgv_group_norm_act_f8(x.data_ptr(), code, N, P, C, groups, _p(weight), _p(bias), eps, act, slope,
+                                                     F8_FORMATS[fmt][0], t.q.data_ptr(), t.scale.data_ptr(), _p(ws), nbytes,
+                                                     stream), "pgv_group_norm_act_f8")
+    return t
+
+
+def group_norm_act_bwd(gy, x, mean, rstd, groups, weight=None, bias=None, act=PGV_ACT_NONE, slope=0.0, need_params=True,
+                       ggamma=None, gbeta=None):
+    """Backward of ``group_norm_act_fwd``: (gx in the type of x, ggamma, gbeta float32 [channels]); the parameter gradients are
+    None without ``need_params``, and written into ``ggamma`` / ``gbeta`` where those are given
+    (``pgv_group_norm_act_bwd``)."""
+    who = "group_norm_act_bwd"
+    code, N, P, C = _gn_args(who, x, groups, weight, bias, act, gy, mean, rstd, ggamma, gbeta)
+    if gy.shape != x.shape or gy.dtype != x.dtype or not gy.is_contiguous():
+        raise ValueError(f"{who}: gy must be like x ({x.dtype}, {tuple(x.shape)}, contiguous)")
+    _f32_vector(who, "mean", mean, N * groups)
+    _f32_vector(who, "rstd", rstd, N * groups)
+    _f32_vector(who, "ggamma", ggamma, C)
+    _f32_vector(who, "gbeta", gbeta, C)
+    gx = torch.empty_like(x)
+    if need_params:
+        ggamma = torch.empty(C, dtype=torch.float32, device=x.device) if ggamma is None else ggamma
+        gbeta = torch.empty(C, dtype=torch.float32, device=x.device) if gbeta is None else gbeta
+    else:
+        ggamma = gbeta = None
+    if x.numel() == 0:
+        return gx, ggamma.zero_() if need_params else None, gbeta.zero_() if need_params else None
+    nbytes = _gn_ws(N, P, C, groups, code, _GN_BWD)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device)
+    with _on_device(x) as stream:
+        _lib.check(_lib.load().pgv_group_norm_act_bwd(gy.data_ptr(), x.data_ptr(), code, N, P, C, groups, _p(weight), _p(bias),
+                                                      mean.data_ptr(), rstd.data_ptr(), act, slope, gx.data_ptr(), _p(ggamma),
+                                                      _p(gbeta), _p(ws), nbytes, stream), "pgv_group_norm_act_bwd")
+    return gx, ggamma, gbeta

@@ -1,0 +1,446 @@
+"""Block-scaled 8-bit operands: quantisation, the product, the Linear forms built on them - against 64-bit restatements.
+
+Tolerances, from the arithmetic: quantised bytes and scales are defined exactly (equality).  A float32 product adds K products
+that are exact in float32: every addition is off by at most 2^-23 of a partial sum, so an element is off by at most
+(K + 64) 2^-23 sum |terms| (64: the scalings, the joining of splits, the bias).  16-bit outputs come from the 8-bit matrix
+instruction, whose 128-term sums carry 17 bits below the largest product (2^-15 of the norm of a result: twice the 1.4e-5 it shows
+on normal data), rounded once: half a step, finfo.eps / 2, of the value."""
+import pytest
+import torch
+
+from helpers import rel_l2
+
+pytestmark = pytest.mark.gpu
+
+F8 = {'e4m3': (torch.float8_e4m3fn, 448.0), 'e5m2': (torch.float8_e5m2, 57344.0)}
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a ROCm GPU")
+    from preset_gen_vae_amd import _lib, ops as _ops
+    _lib.load()
+    return _ops
+
+
+def features(R, C, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed + 1000003 * R + C)
+    x = torch.randn(R, C, generator=g) * torch.exp(0.7 * torch.randn(C, generator=g))
+    if R > 4:
+        x[R // 3] = 0.0
+    return x.to(dtype)
+
+
+def ref_scales(amax, fmt):
+    """(scale, inverse) of the definition, float32 held in float64."""
+    a = amax.double().clamp_min(2.0 ** -100)
+    ok = torch.isfinite(amax)
+    nan = torch.full_like(a, float('nan'))
+    return torch.where(ok, (a / F8[fmt][1]).float().double(), nan), torch.where(ok, (F8[fmt][1] / a).float().double(), nan)
+
+
+def ref_quantize(x, block, fmt):
+    """CPU restatement: (values of the bytes [R, Kp] float32, scales) of x."""
+    R, C = x.shape
+    kb, rb = -(-C // 128), -(-R // 128)
+    w = torch.zeros(rb * 128, kb * 128)
+    w[:R, :C] = x.float()
+    t = w.view(rb, 128, kb, 128)
+    if block == 'row':
+        amax = t.abs().amax(3, keepdim=True)
+    else:
+        amax = t.abs().amax((1, 3), keepdim=True)
+    s, inv = ref_scales(amax, fmt)
+    v = (t * inv.float()).view(rb * 128, kb * 128)[:R]
+    scale = s.view(rb * 128, kb)[:R].t() if block == 'row' else s.view(rb, kb)
+    return v.to(F8[fmt][0]).float(), scale.float()
+
+
+def same(a, b):
+    return torch.equal(torch.nan_to_num(a, nan=12345.0), torch.nan_to_num(b, nan=12345.0))
+
+
+def check_blocks(t, x, block, fmt):
+    q, s = ref_quantize(x, block, fmt)
+    assert t.q.dtype == F8[fmt][0] and tuple(t.q.shape) == tuple(q.shape) and tuple(t.scale.shape) == tuple(s.shape)
+    assert same(t.q.cpu().float(), q) and same(t.scale.cpu(), s)
+
+
+@pytest.mark.parametrize("fmt", ['e4m3', 'e5m2'])
+def test_every_byte_and_every_tie(ops, fmt):
+    """All finite values of the format, the midpoints between neighbours and the float32 numbers next to those, at scale 1."""
+    v = torch.arange(256, dtype=torch.uint8).view(F8[fmt][0]).float()
+    v = v[torch.isfinite(v)].unique()
+    mid = (v[1:] + v[:-1]) / 2
+    x = torch.cat([v, mid, torch.nextafter(mid, torch.tensor(1e9)), torch.nextafter(mid, torch.tensor(-1e9))])
+    x = torch.nn.functional.pad(x, (0, -x.numel() % 127)).view(-1, 127)
+    x = torch.cat([x, torch.full((x.shape[0], 1), F8[fmt][1])], 1)     # the block's maximum is the format's: scale 1
+    t = ops.fp8_quantize(x.cuda(), 'row', fmt)
+    assert (t.scale == 1.0).all()
+    assert torch.equal(t.q.cpu().float(), x.to(F8[fmt][0]).float())
+
+
+SHAPES = [(1, 1), (1, 128), (2, 127), (3, 129), (5, 1000), (127, 130), (128, 128), (129, 256), (257, 391), (300, 64), (1000, 24),
+          (17, 2500), (640, 1920)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("block", ['row', 'tile'])
+def test_quantize(ops, shape, dtype, block):
+    x = features(*shape, dtype)
+    for fmt in F8:
+        check_blocks(ops.fp8_quantize(x.cuda(), block, fmt), x, block, fmt)
+        t, tt = ops.fp8_quantize_both(x.cuda(), block, fmt)
+        check_blocks(t, x, block, fmt)
+        check_blocks(tt, x.t().contiguous(), block, fmt)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("block", ['row', 'tile'])
+def test_quantize_strides_and_alignment(ops, dtype, block):
+    """Rows further apart than their width, starting anywhere; a row or column of any stride; an overlap is refused."""
+    big = features(150, 400, dtype)
+    dev = big.cuda()
+    for r, c0, c1 in ((0, 0, 300), (1, 1, 290), (3, 8, 264), (0, 5, 133)):
+        for f in (ops.fp8_quantize, lambda *a: ops.fp8_quantize_both(*a)[0]):
+            check_blocks(f(dev[r:, c0:c1], block, 'e4m3'), big[r:, c0:c1], block, 'e4m3')
+    check_blocks(ops.fp8_quantize(dev[::2, :130], block, 'e4m3'), big[::2, :130], block, 'e4m3')
+    check_blocks(ops.fp8_quantize(dev[:, 3:4], block, 'e4m3'), big[:, 3:4], block, 'e4m3')
+    check_blocks(ops.fp8_quantize(dev.as_strided((1, 70), (0, 1)), block, 'e4m3'), big[:1, :70], block, 'e4m3')
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.fp8_quantize(dev.as_strided((5, 70), (10, 1)))
+    with pytest.raises(RuntimeError, match="neighbours"):
+        ops.fp8_quantize(dev.t())
+
+
+@pytest.mark.parametrize("block", ['row', 'tile'])
+def test_quantize_extreme_values(ops, block):
+    """Zeros, denormals, the largest finite numbers; a NaN or an infinity takes its block and no other."""
+    x = features(260, 390, torch.float32)
+    x[0] = 0.0
+    x[1] = 1e-42
+    x[2] = 3.3e38
+    x[3, :128] = 2.0 ** -110
+    x[4, 5] = -3e38
+    x[140, 200] = float('nan')
+    x[141, 201] = float('inf')
+    x[259, 389] = float('-inf')
+    for fmt in F8:
+        t, tt = ops.fp8_quantize_both(x.cuda(), block, fmt)
+        check_blocks(t, x, block, fmt)
+        check_blocks(tt, x.t().contiguous(), block, fmt)
+
+
+def ref_product(a, b, bias=None):
+    """(float64 product of two Fp8Blocks, the sums of the magnitudes of its terms)"""
+    def val(t):
+        q, s = t.q.double().cpu(), t.scale.double().cpu()
+        s = s.t() if t.block == 'row' else s.repeat_interleave(128, 0)[:q.shape[0]]
+        return (q.view(q.shape[0], -1, 128) * s.unsqueeze(-1)).flatten(1)
+    av, bv = val(a), val(b)
+    y, mag = av @ bv.t(), av.abs() @ bv.abs().t()
+    return (y, mag) if bias is None else (y + bias.double().cpu(), mag + bias.double().cpu().abs())
+
+
+def check_product(y, a, b, bias=None):
+    ref, mag = ref_product(a, b, bias)
+    got = y.double().cpu()
+    assert tuple(got.shape) == tuple(ref.shape)
+    if y.dtype == torch.float32:
+        assert ((got - ref).abs() <= (a.cols + 64) * 2.0 ** -23 * mag + 1e-37).all()
+    else:
+        assert rel_l2(got, ref) <= torch.finfo(y.dtype).eps / 2 + 2.0 ** -15
+
+
+MNK = [(1, 1, 1), (1, 16, 128), (1, 130, 4100), (3, 17, 129), (16, 256, 2048), (17, 33, 640), (33, 100, 300), (64, 129, 1000),
+       (65, 64, 128), (100, 1000, 72), (128, 128, 128), (129, 257, 385), (200, 72, 5000), (300, 520, 1408), (257, 1024, 2176),
+       (600, 300, 256), (1030, 520, 640)]
+
+
+@pytest.mark.parametrize("mnk", MNK)
+@pytest.mark.parametrize("out", DTYPES)
+def test_matmul(ops, mnk, out):
+    M, N, K = mnk
+    x, w, bias = features(M, K, torch.float32).cuda(), features(N, K, torch.float32, 7).cuda(), features(1, N, torch.float32, 9)[0].cuda()
+    for fa in F8:
+        a = ops.fp8_quantize(x, 'row', fa)
+        for kind in ('tile', 'row'):
+            b = ops.fp8_quantize(w, kind)
+            y = ops.fp8_matmul(a, b, bias, out)
+            check_product(y, a, b, bias)
+            assert torch.equal(y, ops.fp8_matmul(a, b, bias, out))     # the order of its sums is fixed
+    check_product(ops.fp8_matmul(a, b, None, out), a, b)
+
+
+@pytest.mark.parametrize("mnk", [(5, 100, 300), (40, 70, 5000), (200, 72, 700)])
+def test_matmul_writes_its_output_and_nothing_else(ops, mnk):
+    M, N, K = mnk
+    a, b = ops.fp8_quantize(features(M, K, torch.float32).cuda()), ops.fp8_quantize(features(N, K, torch.float32, 3).cuda(), 'tile')
+    for dt in DTYPES:
+        buf = torch.full((M * N + 512,), 7.0, dtype=dt, device='cuda')
+        y = ops.fp8_matmul(a, b, out_dtype=dt, out=buf[:M * N].view(M, N))
+        assert y.data_ptr() == buf.data_ptr() and (buf[M * N:] == 7.0).all()
+        check_product(y, a, b)
+
+
+def test_matmul_propagates_non_finite_rows(ops):
+    """A NaN or an infinity in row m of the first operand makes row m NaN; one in the second makes its tile's columns NaN; nothing
+    else changes."""
+    for M in (7, 150):
+        x, w = features(M, 300, torch.float32), features(260, 300, torch.float32, 3)
+        clean = ops.fp8_matmul(ops.fp8_quantize(x.cuda()), ops.fp8_quantize(w.cuda(), 'tile'), out_dtype=torch.float32)
+        x2, w2 = x.clone(), w.clone()
+        x2[3, 200] = float('inf')
+        w2[129, 0] = float('nan')
+        y = ops.fp8_matmul(ops.fp8_quantize(x2.cuda()), ops.fp8_quantize(w2.cuda(), 'tile'), out_dtype=torch.float32)
+        bad = torch.zeros(M, 260, dtype=torch.bool, device='cuda')
+        bad[3] = True
+        bad[:, 128:256] = True
+        assert torch.equal(torch.isnan(y), bad) and torch.equal(y[~bad], clean[~bad])
+
+
+def test_matmul_empty(ops):
+    bias = torch.arange(5.0, device='cuda')
+    def blocks(R, C):
+        return ops.fp8_quantize(torch.ones(R, C, device='cuda'))
+    assert ops.fp8_matmul(blocks(0, 40), blocks(5, 40), bias).shape == (0, 5)
+    assert ops.fp8_matmul(blocks(4, 40), blocks(0, 40)).shape == (4, 0)
+    assert torch.equal(ops.fp8_matmul(blocks(3, 0), blocks(5, 0), bias, torch.float32), bias.expand(3, 5))
+    assert ops.fp8_linear(torch.ones(0, 40, device='cuda'), ops.fp8_quantize(torch.ones(5, 40, device='cuda'), 'tile'), bias).shape == (0, 5)
+
+
+def test_matmul_beyond_32_bits(ops):
+    """An operand of more than 2^32 bytes: offsets of its last rows do not fit 32 bits."""
+    N, K, M = 66000, 66048, 3
+    q = torch.randint(0, 120, (N, K), dtype=torch.uint8, device='cuda').view(torch.float8_e4m3fn)
+    for kind in ('tile', 'row'):
+        s = torch.rand(*((-(-N // 128), K // 128) if kind == 'tile' else (K // 128, N)), device='cuda') + 0.5
+        b = ops.Fp8Blocks(q, s, kind, K)
+        a = ops.fp8_quantize(features(M, K, torch.float32).cuda())
+        y = ops.fp8_matmul(a, b, out_dtype=torch.float32)
+        pick = torch.tensor([0, 127, 128, 32767, 65023, 65024, 65535, 65999], device='cuda')
+        rows = q.view(torch.uint8)[pick].view(torch.float8_e4m3fn).double()
+        sc = s.double()[pick // 128] if kind == 'tile' else s.double()[:, pick].t()
+        av = ref_val_rows(a)
+        bv = (rows.view(len(pick), -1, 128) * sc.unsqueeze(-1)).flatten(1)
+        ref, mag = av @ bv.t(), av.abs() @ bv.abs().t()
+        assert ((y[:, pick].double() - ref).abs() <= (K + 64) * 2.0 ** -23 * mag).all()
+
+
+def ref_val_rows(t):
+    return (t.q.double().view(t.q.shape[0], -1, 128) * t.scale.double().t().unsqueeze(-1)).flatten(1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("mnk", [(1, 100, 130), (1, 4096, 1024), (5, 257, 1000), (16, 64, 2048), (17, 64, 2048), (33, 130, 24576),
+                                 (64, 100, 999), (65, 100, 999), (200, 300, 520)])
+def test_linear_equals_its_two_steps(ops, mnk, dtype):
+    M, N, K = mnk
+    x, bias = features(M, K, dtype).cuda(), features(1, N, torch.float32, 2)[0].cuda()
+    for kind in ('tile', 'row'):
+        w = ops.fp8_quantize(features(N, K, torch.float32, 5).cuda(), kind)
+        a = ops.fp8_quantize(x)
+        for out in (None, torch.float32, torch.bfloat16):
+            y = ops.fp8_linear(x, w, bias, out)
+            assert y.dtype == (dtype if out is None else out)
+            check_product(y, a, w, bias)
+            assert torch.equal(y, ops.fp8_matmul(a, w, bias, y.dtype))
+    wide = torch.zeros(M, K + 3, dtype=dtype, device='cuda')
+    wide[:, 1:K + 1] = x
+    assert torch.equal(ops.fp8_linear(wide[:, 1:K + 1], w, bias), ops.fp8_linear(x, w, bias))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("mnk", [(1, 3, 5), (7, 100, 300), (130, 257, 391), (256, 130, 1000), (600, 96, 64)])
+@pytest.mark.parametrize("grad_fmt", ['e4m3', 'e5m2'])
+def test_linear_gradients_against_the_formula(ops, mnk, dtype, grad_fmt):
+    M, N, K = mnk
+    x, w, b, gy = features(M, K, dtype), features(N, K, torch.float32, 4), features(1, N, torch.float32, 6)[0], features(M, N, dtype, 8)
+    y, saved = ops.fp8_linear_fwd(x.cuda(), w.cuda(), b.cuda())
+    gx, gw, gb = ops.fp8_linear_bwd(gy.cuda(), saved, grad_fmt)
+    a, wt = ops.fp8_quantize(x.cuda()), ops.fp8_quantize(w.cuda(), 'tile')
+    check_product(y, a, wt, b)
+    g, gt = ops.fp8_quantize(gy.cuda(), 'row', grad_fmt), ops.fp8_quantize(gy.t().contiguous().cuda(), 'row', grad_fmt)
+    check_product(gx, g, ops.fp8_quantize(w.t().contiguous().cuda(), 'tile'))
+    check_product(gw, gt, ops.fp8_quantize(x.t().contiguous().cuda()))
+    assert gx.dtype == dtype and gw.dtype == torch.float32 and gb.dtype == torch.float32
+    # column sums: M additions in float32 of exact values
+    ref = gy.double().sum(0)
+    assert ((gb.double().cpu() - ref).abs() <= M * 2.0 ** -23 * gy.double().abs().sum(0) + 1e-37).all()
+    for need in ((True, False, False), (False, True, False), (False, False, True), (False, False, False)):
+        part = ops.fp8_linear_bwd(gy.cuda(), saved, grad_fmt, need)
+        for p, full, n in zip(part, (gx, gw, gb), need):
+            assert (p is None) == (not n) and (p is None or torch.equal(p, full))
+
+
+def test_linear_gradients_against_differences(ops):
+    """The products are linear in the values the operands stand for, so a difference over any step is the derivative: with an
+    output gradient that 8 bits hold exactly, <gx, d> and <gw, d> are the differences of <gy, y>."""
+    M, N, K = 70, 130, 200
+    x, w = features(M, K, torch.float32), features(N, K, torch.float32, 4)
+    g = torch.Generator().manual_seed(3)
+    gy = torch.randint(-2, 3, (M, N), generator=g).float()
+    gy[0] = 2.0           # every block of 128, along rows and columns, has its maximum at 2: values 0, 1, 2 are exact
+    gy[:, ::64] = 2.0
+    y, saved = ops.fp8_linear_fwd(x.cuda(), w.cuda())
+    gx, gw, gb = ops.fp8_linear_bwd(gy.cuda(), saved)
+    assert gb is None
+    xv, wv = ops.fp8_quantize(x.cuda()).dequantize().double().cpu(), ops.fp8_quantize(w.cuda(), 'tile').dequantize().double().cpu()
+    xcol = ops.fp8_quantize(x.t().contiguous().cuda()).dequantize().t().double().cpu()     # what the weight gradient reads
+    d, dw = torch.randn(M, K, generator=g).double(), torch.randn(N, K, generator=g).double()
+    loss = lambda a, b: (gy.double() * (a @ b.t())).sum()  # noqa: E731
+    h = 0.5
+    diff = (loss(xv + h * d, wv) - loss(xv - h * d, wv)) / (2 * h)
+    scale = (gx.double().cpu().abs() * d.abs()).sum()
+    assert abs((gx.double().cpu() * d).sum() - diff) <= (N + 64) * 2.0 ** -23 * (gy.double().abs() @ wv.abs() * d.abs()).sum() + 1e-9 * scale
+    diff = (loss(xcol, wv + h * dw) - loss(xcol, wv - h * dw)) / (2 * h)
+    assert abs((gw.double().cpu() * dw).sum() - diff) <= (M + 64) * 2.0 ** -23 * (gy.double().abs().t() @ xcol.abs() * dw.abs()).sum()
+
+
+def test_other_streams_and_captured_calls(ops):
+    """A call on another stream; two captured graphs, replayed in turn with eager calls between, each replay against the eager
+    result on the same values."""
+    N, K = 260, 1500
+    w = ops.fp8_quantize(features(N, K, torch.float32, 5).cuda(), 'tile')
+    wm = features(N, K, torch.float32, 5).cuda()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        xs = features(40, K, torch.bfloat16, 1).cuda()
+        ys = ops.fp8_linear(xs, w)
+    side.synchronize()
+    assert torch.equal(ys, ops.fp8_linear(xs, w))
+    graphs = []
+    for M in (9, 40, 150):
+        x = torch.zeros(M, K, dtype=torch.bfloat16, device='cuda')
+        gy = torch.zeros(M, N, dtype=torch.bfloat16, device='cuda')
+
+        def step(x=x, gy=gy):
+            y, saved = ops.fp8_linear_fwd(x, wm)
+            return (ops.fp8_linear(x, w), y) + ops.fp8_linear_bwd(gy, saved)[:2]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, x, gy, step, out))
+    for rep in range(3):
+        for graph, x, gy, step, out in graphs:
+            x.copy_(features(*x.shape, torch.bfloat16, rep))
+            gy.copy_(features(*gy.shape, torch.bfloat16, rep + 50))
+        for graph, *_ in graphs:
+            graph.replay()
+        for graph, x, gy, step, out in graphs:
+            for a, b in zip(out, step()):
+                assert torch.equal(a, b)
+
+
+def test_refusals(ops):
+    x = features(8, 256, torch.float32).cuda()
+    a, b = ops.fp8_quantize(x), ops.fp8_quantize(x, 'tile')
+    with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
+        ops.fp8_quantize(x.double())
+    with pytest.raises(ValueError, match="'row' or 'tile'"):
+        ops.fp8_quantize(x, 'column')
+    with pytest.raises(ValueError, match="2-d"):
+        ops.fp8_quantize(x[0])
+    with pytest.raises(TypeError, match="Fp8Blocks"):
+        ops.fp8_matmul(x, b)
+    with pytest.raises(ValueError, match="'row' blocks"):
+        ops.fp8_matmul(b, b)
+    with pytest.raises(ValueError, match="must be e4m3"):
+        ops.fp8_matmul(a, ops.fp8_quantize(x, 'row', 'e5m2'))
+    with pytest.raises(ValueError, match="reductions"):
+        ops.fp8_matmul(a, ops.fp8_quantize(x[:, :200], 'tile'))
+    with pytest.raises(ValueError, match="bias"):
+        ops.fp8_matmul(a, b, torch.zeros(9, device='cuda'))
+    with pytest.raises(ValueError, match="output type"):
+        ops.fp8_matmul(a, b, out_dtype=torch.float64)
+    with pytest.raises(ValueError, match="out must be"):
+        ops.fp8_matmul(a, b, out=torch.zeros(8, 9, device='cuda', dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="scales of shape|scale must be"):
+        ops.fp8_matmul(a._replace(scale=a.scale.t().contiguous()), b)
+    with pytest.raises(ValueError, match="rows of"):
+        ops.fp8_matmul(a._replace(cols=300), b)
+    with pytest.raises(RuntimeError, match="different devices"):
+        ops.fp8_matmul(a, b, torch.zeros(8))
+    with pytest.raises(RuntimeError, match="16-byte aligned"):
+        ops.fp8_matmul(a, b, out_dtype=torch.float32, out=torch.zeros(65, device='cuda')[1:].view(8, 8))
+    with pytest.raises(ValueError, match="features"):
+        ops.fp8_linear(x[:, :200], b)
+    with pytest.raises(ValueError, match="do not match"):
+        ops.fp8_linear_fwd(x, x[:, :200])
+    with pytest.raises(ValueError, match="expected"):
+        ops.fp8_linear_bwd(x, ops.fp8_linear_fwd(x, x)[1])
+
+
+# ---- the module and the path that uses it ----------------------------------------------------------------------------------
+def test_module_trains_and_serves(ops):
+    from preset_gen_vae_amd.model import layer
+    torch.manual_seed(1)
+    lin = layer.Fp8Linear(300, 130).cuda()
+    assert sorted(lin.state_dict()) == ['bias', 'weight']
+    x = features(6, 300, torch.float32).cuda().view(2, 3, 300).requires_grad_(True)
+    gy = features(6, 130, torch.float32, 2).cuda().view(2, 3, 130)
+    y = lin(x)
+    y.backward(gy)
+    yr, saved = ops.fp8_linear_fwd(x.detach().view(6, 300), lin.weight.detach(), lin.bias.detach())
+    gx, gw, gb = ops.fp8_linear_bwd(gy.view(6, 130), saved)
+    assert torch.equal(y.view(6, 130), yr) and torch.equal(x.grad.view(6, 300), gx)
+    assert torch.equal(lin.weight.grad, gw) and torch.equal(lin.bias.grad, gb)
+    with torch.no_grad():
+        lin.eval()
+        plain = lin(x)
+        assert torch.equal(plain, lin.quantize_weight()(x)) and rel_l2(plain.view(6, 130), yr) < 1e-6
+        lin.weight.mul_(2.0)
+        lin.load_state_dict(lin.state_dict())         # a reloaded weight is not served from the old layout
+        assert rel_l2(lin(x) - lin.bias, 2 * (plain - lin.bias)) < 1e-5
+    lin.quantize_weight().train()
+    assert lin._weight8 is None
+    frozen = layer.Fp8Linear(300, 130).cuda()
+    frozen.weight.requires_grad_(False)
+    frozen(x.detach().requires_grad_(True)).sum().backward()
+    assert frozen.weight.grad is None and frozen.bias.grad is not None
+
+
+def test_module_in_flat_parameters(ops):
+    """Gradients written into the flat buffer: one application per step, two applications, a second backward without a clearing -
+    against ordinary autograd accumulation."""
+    from preset_gen_vae_amd.model import layer
+    from preset_gen_vae_amd.optim import FlatParams, FusedAdam
+    torch.manual_seed(2)
+    net, ref = layer.Fp8Linear(128, 128).cuda(), layer.Fp8Linear(128, 128).cuda()
+    ref.load_state_dict(net.state_dict())
+    opt = FusedAdam(FlatParams(net.parameters()))
+    x = features(20, 128, torch.float32).cuda()
+    for twice, passes in ((False, 1), (True, 1), (False, 2)):
+        opt.zero_grad()
+        ref.zero_grad()
+        for m in (net, ref):
+            for _ in range(passes):
+                h = m(x)
+                (m(h) if twice else h).square().sum().backward()
+        assert rel_l2(net.weight.grad, ref.weight.grad) < 1e-6 and rel_l2(net.bias.grad, ref.bias.grad) < 1e-6
+
+
+@pytest.mark.parametrize("arch", ['3l128_fp8', '3l128_gn', '3l128_gn_fp8'])
+def test_regression_suffixes(ops, arch):
+    """The regression MLP with its suffixes runs forward and backward; its gradients are near the plain network's where only the
+    operand precision differs (8-bit rounding: 2^-4 per operand value)."""
+    from preset_gen_vae_amd.model.regression import MLPRegression
+
+    class Helper:
+        learnable_preset_size = 21
+    torch.manual_seed(0)
+    net = MLPRegression(arch, 64, Helper()).cuda()
+    z = features(9, 64, torch.float32).cuda()
+    out = net(z)
+    assert out.shape == (9, 21)
+    out.sum().backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in net.parameters())
+    keys = ''.join(net.state_dict())
+    assert ('gn1' in keys) == ('gn' in arch) and ('bn1' in keys) == ('gn' not in arch)
