@@ -86,35 +86,49 @@ struct skinny_args {
   float* part;            // [splits][M][N] when splits > 1
 };
 
-// 32 consecutive values of a row as 32 bytes + their block's scale
+// 32 consecutive values of a row, as they lie in memory (VEC: 16-byte aligned), then as 32 bytes + their block's scale
+template <typename T>
+struct raw32 {
+  T v[32];
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void quant_frag(const T* __restrict__ p, int n, bool row_ok, i32x8& f, float& scale) {
-  float v[32];
+__device__ __forceinline__ raw32<T> load32(const T* __restrict__ p, int n) {
+  raw32<T> r;
+  constexpr int E = 16 / sizeof(T);
+  typedef T te __attribute__((ext_vector_type(E)));
+  if (VEC && n >= 32) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float t[8];
-    if (row_ok)
-      f8_load8<VEC>(p + 8 * i, n - 8 * i, t);
-    else
+    for (int i = 0; i < 32 / E; ++i) {
+      const te t = reinterpret_cast<const te*>(p)[i];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = 0.f;
+      for (int j = 0; j < E; ++j) r.v[i * E + j] = t[j];
+    }
+  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[8 * i + j] = t[j];
+    for (int i = 0; i < 32; ++i) r.v[i] = i < n ? p[i] : (T)0.f;
   }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ i32x8 quant_frag(const raw32<T>& r, float& scale) {
+  i32x8 f;
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) m = max(m, f8_abs_bits(v[i]));
+  for (int i = 0; i < 32; ++i) m = max(m, f8_abs_bits((float)r.v[i]));
   m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
   m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
   float inv;
   f8_scale<PGV_F8_E4M3>(m, scale, inv);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    f[i] = f8_pack4<PGV_F8_E4M3>(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv, v[4 * i + 3] * inv);
+    f[i] = f8_pack4<PGV_F8_E4M3>((float)r.v[4 * i] * inv, (float)r.v[4 * i + 1] * inv, (float)r.v[4 * i + 2] * inv,
+                                 (float)r.v[4 * i + 3] * inv);
+  return f;
 }
 
-// T = uint8_t: a is 8-bit rows of format FA; else its values are quantised here (e4m3).  MF x NF tiles of 16 x 16 per wave.
-template <typename T, int FA, bool F32, bool VEC, int MF, int NF>
+// T = uint8_t: a is 8-bit rows of format FA; else its values are quantised here (e4m3).  MF x NF tiles of 16 x 16 per wave;
+// U blocks of the reduction are requested before the first is used: a wave has few of them, so their latencies must overlap.
+template <typename T, int FA, bool F32, bool VEC, int MF, int NF, int U>
 __global__ __launch_bounds__(64 * SW) void skinny_kernel(skinny_args p) {
   constexpr bool Q = sizeof(T) == 1;
   constexpr int GRP = NF * MF < 4 ? NF * MF : 4;   // tiles that meet in LDS at a time
@@ -137,39 +151,55 @@ __global__ __launch_bounds__(64 * SW) void skinny_kernel(skinny_args p) {
   for (int f = 0; f < NF; ++f)
 #pragma unroll
     for (int i = 0; i < MF; ++i) acc[f][i] = {0.f, 0.f, 0.f, 0.f};
-  for (int kb = kb0 + wave; kb < kb1; kb += SW) {
-    frag<F32> bf[NF], af[MF];
-    float sbv[NF], sav[MF];
+  for (int kbase = kb0 + wave; kbase < kb1; kbase += SW * U) {
+    i32x8 b8[U][NF], a8[U][Q ? MF : 1];
+    raw32<T> av[U][Q ? 1 : MF];
+    float sb[U][NF], sa[U][MF];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
-      const i32x4* s = reinterpret_cast<const i32x4*>(bp[f] + (int64_t)kb * F8B);
-      bf[f] = make_frag<PGV_F8_E4M3, F32>(cat8(s[0], s[1]));
-      sbv[f] = sbp[f][kb];
-    }
+    for (int u = 0; u < U; ++u) {
+      // (a block past the end is read as the last one and takes no part)
+      const int kb = min(kbase + u * SW, kb1 - 1);
 #pragma unroll
-    for (int i = 0; i < MF; ++i) {
-      const int m = m0 + 16 * i + l16;
-      if constexpr (Q) {
-        const int mc = min(m, p.M - 1);
-        const i32x4* s = reinterpret_cast<const i32x4*>((const uint8_t*)p.a + mc * Kp + (int64_t)kb * F8B + g * 32);
-        af[i] = make_frag<FA, F32>(cat8(s[0], s[1]));
-        sav[i] = p.sa[(int64_t)kb * p.M + mc];
-      } else {
-        const int k = kb * F8B + g * 32;
-        i32x8 bytes;
-        quant_frag<T, VEC>((const T*)p.a + m * p.lda + k, p.K - k, m < p.M, bytes, sav[i]);
-        af[i] = make_frag<PGV_F8_E4M3, F32>(bytes);
+      for (int f = 0; f < NF; ++f) {
+        const i32x4* s = reinterpret_cast<const i32x4*>(bp[f] + (int64_t)kb * F8B);
+        b8[u][f] = cat8(s[0], s[1]);
+        sb[u][f] = sbp[f][kb];
       }
-    }
-#pragma unroll
-    for (int f = 0; f < NF; ++f)
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
-        const f32x4 d = mfma128<FA, F32>(bf[f], af[i]);
-        const float s = sav[i] * sbv[f];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[f][i][j] = fmaf(d[j], s, acc[f][i][j]);
+        const int mc = min(m0 + 16 * i + l16, p.M - 1);
+        if constexpr (Q) {
+          const i32x4* s = reinterpret_cast<const i32x4*>((const uint8_t*)p.a + mc * Kp + (int64_t)kb * F8B + g * 32);
+          a8[u][i] = cat8(s[0], s[1]);
+          sa[u][i] = p.sa[(int64_t)kb * p.M + mc];
+        } else {
+          const int k = kb * F8B + g * 32;
+          av[u][i] = load32<T, VEC>((const T*)p.a + mc * p.lda + k, p.K - k);
+        }
       }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (kbase + u * SW >= kb1) break;
+      frag<F32> bf[NF];
+#pragma unroll
+      for (int f = 0; f < NF; ++f) bf[f] = make_frag<PGV_F8_E4M3, F32>(b8[u][f]);
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        frag<F32> af;
+        if constexpr (Q)
+          af = make_frag<FA, F32>(a8[u][i]);
+        else
+          af = make_frag<PGV_F8_E4M3, F32>(quant_frag(av[u][i], sa[u][i]));
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+          const f32x4 d = mfma128<FA, F32>(bf[f], af);
+          const float s = sa[u][i] * sb[u][f];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[f][i][j] = fmaf(d[j], s, acc[f][i][j]);
+        }
+      }
+    }
   }
   // the waves' sums meet, GRP tiles at a time: image [wave][tile][m 16][n 16]
 #pragma unroll
@@ -383,10 +413,10 @@ int launch_tile(tile_args p, hipStream_t st) {
   return PGV_OK;
 }
 
-template <typename T, int FA, bool F32, bool VEC, int MF, int NF>
+template <typename T, int FA, bool F32, bool VEC, int MF, int NF, int U>
 void launch_skinny(const skinny_args& p, hipStream_t st) {
-  skinny_kernel<T, FA, F32, VEC, MF, NF><<<dim3((unsigned)pgv_cdiv(p.N, 16 * NF), (unsigned)pgv_cdiv(p.M, 16 * MF), (unsigned)p.splits),
-                                      64 * SW, 0, st>>>(p);
+  skinny_kernel<T, FA, F32, VEC, MF, NF, U>
+      <<<dim3((unsigned)pgv_cdiv(p.N, 16 * NF), (unsigned)pgv_cdiv(p.M, 16 * MF), (unsigned)p.splits), 64 * SW, 0, st>>>(p);
 }
 
 // ---- which kernel, and how the reduction is split: a function of the sizes alone -------------------------------------------
@@ -402,7 +432,7 @@ plan make_plan(int64_t M, int64_t N, int64_t Kb, int b_block) {
   int64_t wgs;
   int64_t most;
   if (q.skinny) {
-    q.mf = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    q.mf = M <= 16 ? 1 : M <= 32 ? 2 : M <= 48 ? 3 : 4;
     q.nf = 1;
     wgs = pgv_cdiv(N, 16 * q.nf);
     most = Kb / (2 * SW);
@@ -436,11 +466,13 @@ int run_matmul(int64_t M, int64_t N, int64_t K, const void* a, const float* sa, 
   if (pl.skinny) {
     skinny_args p = {(int)M, (int)N, (int)K, Kb, pl.splits, a, 0, sa, (const uint8_t*)b, sb, bias, out, out_dt, part};
     if (pl.mf == 1)
-      launch_skinny<uint8_t, FA, F32, true, 1, 1>(p, st);
+      launch_skinny<uint8_t, FA, F32, true, 1, 1, 4>(p, st);
     else if (pl.mf == 2)
-      launch_skinny<uint8_t, FA, F32, true, 2, 1>(p, st);
+      launch_skinny<uint8_t, FA, F32, true, 2, 1, 4>(p, st);
+    else if (pl.mf == 3)
+      launch_skinny<uint8_t, FA, F32, true, 3, 1, 3>(p, st);
     else
-      launch_skinny<uint8_t, FA, F32, true, 4, 1>(p, st);
+      launch_skinny<uint8_t, FA, F32, true, 4, 1, 2>(p, st);
   } else {
     tile_args p = {(int)M, (int)N, Kb, pl.splits, 0, 0, (const uint8_t*)a, sa, (const uint8_t*)b, sb, bias, out, out_dt, part};
     const int rc = b_block == PGV_F8_ROWS ? launch_tile<128, 128, 64, 64, true, FA, F32>(p, st) : launch_tile<128, 128, 64, 64, false, FA, F32>(p, st);
@@ -513,7 +545,8 @@ extern "C" int pgv_f8_linear(const void* x, int dtype, int64_t M, int64_t K, int
   hipStream_t st = pgv_stream(stream);
   skinny_args p = {(int)M, (int)N, (int)K, Kb, pl.splits, x, ldx, nullptr, (const uint8_t*)b, b_scale, bias, out, out_dtype, (float*)workspace};
   const bool vec = (uintptr_t)x % 16 == 0 && (ldx * f8_dt_size(dtype)) % 16 == 0;
-#define PGV_SK2(T, F32) (vec ? launch_skinny<T, 0, F32, true, 1, 1>(p, st) : launch_skinny<T, 0, F32, false, 1, 1>(p, st))
+#define PGV_SK2(T, F32) \
+  (vec ? launch_skinny<T, 0, F32, true, 1, 1, sizeof(T) == 4 ? 2 : 4>(p, st) : launch_skinny<T, 0, F32, false, 1, 1, 1>(p, st))
 #define PGV_SK(T) (out_dtype == PGV_DT_F32 ? PGV_SK2(T, true) : PGV_SK2(T, false))
   if (dtype == PGV_DT_F32)
     PGV_SK(float);

@@ -64,29 +64,50 @@ __device__ __forceinline__ void act_grad8(float (&g)[8], const float (&u)[8], in
   }
 }
 
-// 8 neighbouring values as they lie in memory
+// 8 neighbouring values as they lie in memory: 16-bit types stay two to a register until they are used
 template <typename T>
 struct raw8 {
-  T v[8];
+  static constexpr int WORDS = 2 * sizeof(T);
+  uint32_t w[WORDS];
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else if constexpr (__is_same(T, __bf16)) {
+      return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    } else {
+      return (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]));
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = 0;
+  }
+  // the compiler forgets what it derived from the words: the widened values of one pass are not kept for the next
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) asm volatile("" : "+v"(w[i]));
+  }
 };
 template <bool VEC, typename T>
 __device__ __forceinline__ raw8<T> load_raw(const T* __restrict__ p, int n) {
   raw8<T> r;
   if constexpr (VEC) {
-    typedef T t8 __attribute__((ext_vector_type(8)));
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    if constexpr (sizeof(T) == 4) {
-      const t4 a = reinterpret_cast<const t4*>(p)[0], b = reinterpret_cast<const t4*>(p)[1];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r.v[i] = a[i], r.v[4 + i] = b[i];
-    } else {
-      const t8 a = *reinterpret_cast<const t8*>(p);
+    for (int h = 0; h < r.WORDS / 4; ++h) {
+      const i32x4 a = reinterpret_cast<const i32x4*>(p)[h];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r.v[i] = a[i];
+      for (int i = 0; i < 4; ++i) r.w[4 * h + i] = (uint32_t)a[i];
     }
   } else {
+    r.clear();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = i < n ? p[i] : (T)0.f;
+    for (int i = 0; i < 8; ++i) {
+      if (i >= n) continue;
+      if constexpr (sizeof(T) == 4)
+        r.w[i] = __float_as_uint((float)p[i]);
+      else
+        r.w[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << (i & 1 ? 16 : 0);
+    }
   }
   return r;
 }
@@ -113,46 +134,56 @@ __device__ __forceinline__ void store8(T* __restrict__ p, int n, const float (&v
   }
 }
 
-// One thread's place: 8 channels from c, valid ones n (0: a pad column of the 8-bit rows or an idle thread), pixel phase r.
+// One thread's place: 8 channels from c, valid ones n (0: a pad column of the 8-bit rows or an idle thread), pixel phase r of rpp.
+// SAME (C/G a multiple of 8): the 8 channels are of one group g[0], and mean, rstd and the like are one register each.
+template <bool SAME>
 struct place {
+  static constexpr int A = SAME ? 1 : 8;
   int c, n, r, rpp;
+  int g[A];   // groups of the channels within the item
 };
-__device__ __forceinline__ place my_place(const gn_args& p, int c0, int nt) {
-  place q;
-  const int j = threadIdx.x % p.tpr;
+template <bool SAME>
+__device__ __forceinline__ place<SAME> my_place(const gn_args& p, int c0, int nt) {
+  place<SAME> q;
+  const int row = threadIdx.x / p.tpr, j = threadIdx.x - row * p.tpr;
   q.rpp = nt / p.tpr;
-  q.r = threadIdx.x / p.tpr;
+  q.r = row;
   q.c = c0 + 8 * j;
   const int end = min(c0 + p.W, p.C);
   q.n = q.r < q.rpp ? max(0, min(8, end - q.c)) : 0;
+#pragma unroll
+  for (int i = 0; i < q.A; ++i) q.g[i] = i < q.n ? (q.c + i) / p.cg : 0;
   return q;
 }
 // the per-channel vectors of a place; channels beyond the valid ones normalise to 0
+template <bool SAME>
 struct chan {
-  float ga[8], be[8], mu[8], rs[8];
+  float ga[8], be[8], mu[SAME ? 1 : 8], rs[SAME ? 1 : 8];
 };
-__device__ __forceinline__ void load_affine(const gn_args& p, const place& q, chan& k) {
+template <bool SAME>
+__device__ __forceinline__ void load_affine(const gn_args& p, const place<SAME>& q, chan<SAME>& k) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     k.ga[i] = i < q.n && p.gamma ? p.gamma[q.c + i] : (i < q.n ? 1.f : 0.f);
     k.be[i] = i < q.n && p.beta ? p.beta[q.c + i] : 0.f;
   }
 }
-__device__ __forceinline__ void load_stats(const gn_args& p, const place& q, int item, chan& k) {
+template <bool SAME>
+__device__ __forceinline__ void load_stats(const gn_args& p, const place<SAME>& q, int item, chan<SAME>& k) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t g = (int64_t)item * p.G + (i < q.n ? (q.c + i) / p.cg : 0);
+  for (int i = 0; i < q.A; ++i) {
+    const int64_t g = (int64_t)item * p.G + q.g[i];
     k.mu[i] = i < q.n ? p.mean[g] : 0.f;
     k.rs[i] = i < q.n ? p.rstd[g] : 0.f;
   }
 }
 
 // y (or its 8-bit block) of one pixel
-template <bool VEC, bool Q, int FMT, typename T>
-__device__ __forceinline__ void put(const gn_args& p, const place& q, const chan& k, int64_t pix, const raw8<T>& x) {
+template <bool VEC, bool Q, int FMT, bool SAME, typename T>
+__device__ __forceinline__ void put(const gn_args& p, const place<SAME>& q, const chan<SAME>& k, int64_t pix, const raw8<T>& x) {
   float u[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) u[i] = fmaf(((float)x.v[i] - k.mu[i]) * k.rs[i], k.ga[i], k.be[i]);
+  for (int i = 0; i < 8; ++i) u[i] = fmaf((x[i] - k.mu[SAME ? 0 : i]) * k.rs[SAME ? 0 : i], k.ga[i], k.be[i]);
   act8(u, p.act, p.slope);
   if constexpr (!Q) {
     store8<VEC>((T*)p.y + pix * p.C + q.c, q.n, u);
@@ -171,41 +202,53 @@ __device__ __forceinline__ void put(const gn_args& p, const place& q, const chan
   }
 }
 
-// sums over (pixel phases x channels) of each local group: val[tid][8] in LDS -> out[group]
-__device__ __forceinline__ void group_sums(const gn_args& p, const float* val, int tpr, int rpp, int groups, float* out) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  for (int g = wave; g < groups; g += nw) {
-    float s = 0.f;
-    for (int e = lane; e < rpp * p.cg; e += 64) {
-      const int r = e / p.cg, c = g * p.cg + e % p.cg;
-      s += val[r * tpr * 8 + c];
-    }
-    s = pgv_wave_sum(s);
-    if (lane == 0) out[g] = s;
+// Sums over the entries of every group: L neighbouring lanes per group (a power of two, at most 64), each over every L-th entry.
+// at(g, e): entry e < cnt(g) of local group g; done(g, sum): called by one lane.
+template <typename V, typename At, typename Cnt, typename Done>
+__device__ __forceinline__ void sum_groups(int groups, int nt, At at, Cnt cnt, Done done) {
+  int lg = 31 - __builtin_clz(max(1, nt / groups));
+  lg = lg > 6 ? 6 : lg;
+  const int L = 1 << lg, s = threadIdx.x & (L - 1);
+  for (int g = threadIdx.x >> lg; g < ((groups + (nt >> lg) - 1) / (nt >> lg)) * (nt >> lg); g += nt >> lg) {
+    V v{};
+    const int n = g < groups ? cnt(g) : 0;
+    for (int e = s; e < n; e += L) v.add(at(g, e));
+    for (int o = L >> 1; o > 0; o >>= 1) v.add(v.from(o));
+    if (s == 0 && g < groups) done(g, v);
   }
 }
-// the same for groups of whole 8-channel pieces: val[tid] is the sum of a thread's channels
-__device__ __forceinline__ void group_sums8(const gn_args& p, const float* val, int tpr, int rpp, int groups, float* out) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6, per = p.cg >> 3;
-  for (int g = wave; g < groups; g += nw) {
-    float s = 0.f;
-    for (int e = lane; e < rpp * per; e += 64) s += val[(e / per) * tpr + g * per + e % per];
-    s = pgv_wave_sum(s);
-    if (lane == 0) out[g] = s;
+struct sum1 {
+  float a;
+  __device__ __forceinline__ void add(const sum1& o) { a += o.a; }
+  __device__ __forceinline__ sum1 from(int o) const {
+    sum1 r;
+    r.a = __shfl_xor(a, o, 64);
+    return r;
   }
-}
+};
+template <typename F>
+struct sum2 {
+  F a, b;
+  __device__ __forceinline__ void add(const sum2& o) { a += o.a, b += o.b; }
+  __device__ __forceinline__ sum2 from(int o) const {
+    sum2 r;
+    r.a = __shfl_xor(a, o, 64);
+    r.b = __shfl_xor(b, o, 64);
+    return r;
+  }
+};
 
 constexpr int MAXG = 256;   // groups of a workgroup of the fused kernels
 
 // ---- forward, fused: grid (column blocks of W channels, items) -----------------------------------------------------------
 template <typename T, int NT, int KV, bool VEC, bool Q, int FMT, bool SAME>
 __global__ __launch_bounds__(NT) void gn_fwd_fused_kernel(gn_args p) {
-  __shared__ float val[SAME ? NT : NT * 8];
+  constexpr int A = SAME ? 1 : 8;
+  __shared__ __attribute__((aligned(16))) float val[NT * A];
   __shared__ float gs[2][MAXG];
   const int tid = threadIdx.x, item = blockIdx.y, c0 = blockIdx.x * p.W;
-  const place q = my_place(p, c0, NT);
-  const bool idle = q.r >= q.rpp;
-  const int groups = min(p.W, p.C - c0) / p.cg;
+  const place<SAME> q = my_place<SAME>(p, c0, NT);
+  const int groups = min(p.W, p.C - c0) / p.cg, gfirst = c0 / p.cg;
   const T* x = (const T*)p.x + (int64_t)item * p.P * p.C;
   raw8<T> d[KV];
 #pragma unroll
@@ -214,44 +257,45 @@ __global__ __launch_bounds__(NT) void gn_fwd_fused_kernel(gn_args p) {
     if (r < p.P && q.n > 0)
       d[k] = load_raw<VEC>(x + (int64_t)r * p.C + q.c, q.n);
     else
-#pragma unroll
-      for (int i = 0; i < 8; ++i) d[k].v[i] = (T)0.f;
+      d[k].clear();
   }
-  chan ch;
-  load_affine(p, q, ch);
+  chan<SAME> ch;
   const float inv_n = 1.f / ((float)p.P * (float)p.cg);
+  const int per = SAME ? p.cg >> 3 : p.cg, pitch = SAME ? p.tpr : p.tpr * 8;
   // pass 0: mean; pass 1: variance
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ch.mu[i] = 0.f;
+  for (int i = 0; i < A; ++i) ch.mu[i] = 0.f;
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {
-    float s[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = 0.f;
+    for (int k = 0; k < KV; ++k) d[k].forget();
+    float s[A];
+#pragma unroll
+    for (int i = 0; i < A; ++i) s[i] = 0.f;
 #pragma unroll
     for (int k = 0; k < KV; ++k)
       if (q.r + k * q.rpp < p.P)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float v = (float)d[k].v[i] - ch.mu[i];
-          s[i] += pass ? v * v : v;
+          const float v = d[k][i] - ch.mu[SAME ? 0 : i];
+          s[SAME ? 0 : i] += pass ? v * v : v;
         }
-    if (pass) __syncthreads();   // the readers of val and gs of pass 0 are done
-    if constexpr (SAME) {
-      val[tid] = q.n > 0 ? ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])) : 0.f;
-    } else {
+    if (pass) __syncthreads();   // the readers of val of pass 0 are done
 #pragma unroll
-      for (int i = 0; i < 8; ++i) val[tid * 8 + i] = i < q.n ? s[i] : 0.f;
-    }
+    for (int i = 0; i < A; ++i) val[tid * A + i] = i < q.n ? s[i] : 0.f;
     __syncthreads();
-    if constexpr (SAME)
-      group_sums8(p, val, p.tpr, q.rpp, groups, gs[pass]);
-    else
-      group_sums(p, val, p.tpr, q.rpp, groups, gs[pass]);
+    sum_groups<sum1>(groups, NT,
+        [&](int g, int e) {
+          const int r = e / per;
+          sum1 v;
+          v.a = val[r * pitch + g * per + (e - r * per)];
+          return v;
+        },
+        [&](int) { return q.rpp * per; }, [&](int g, const sum1& v) { gs[pass][g] = v.a; });
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int g = i < q.n ? (q.c + i - c0) / p.cg : 0;
+    for (int i = 0; i < A; ++i) {
+      const int g = i < q.n ? q.g[i] - gfirst : 0;
       if (pass == 0)
         ch.mu[i] = i < q.n ? gs[0][g] * inv_n : 0.f;
       else
@@ -260,31 +304,39 @@ __global__ __launch_bounds__(NT) void gn_fwd_fused_kernel(gn_args p) {
   }
   if (p.mean)
     for (int g = tid; g < groups; g += NT) {
-      const int64_t o = (int64_t)item * p.G + c0 / p.cg + g;
+      const int64_t o = (int64_t)item * p.G + gfirst + g;
       p.mean[o] = gs[0][g] * inv_n;
       p.rstd[o] = 1.f / sqrtf(gs[1][g] * inv_n + p.eps);
     }
-  if (idle) return;
+  if (q.r >= q.rpp) return;
+  load_affine(p, q, ch);
 #pragma unroll
   for (int k = 0; k < KV; ++k) {
     const int r = q.r + k * q.rpp;
+    d[k].forget();
     if (r < p.P && (Q || q.n > 0)) put<VEC, Q, FMT>(p, q, ch, (int64_t)item * p.P + r, d[k]);
   }
 }
 
 // ---- forward, two-pass --------------------------------------------------------------------------------------------------
-// partial sums: part (as double2) [N][slices * column blocks][G] of (sum, sum of squares), zero for groups outside the block
+// partial sums: part (as sum2<double>) [N][column blocks * slices][G] of (sum, sum of squares), zero for groups outside the block
 template <typename T, bool VEC, bool SAME>
 __global__ __launch_bounds__(256) void gn_stats_kernel(gn_args p) {
-  __shared__ double2 val[SAME ? 256 : 2048];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, item = blockIdx.z, slice = blockIdx.x, c0 = blockIdx.y * p.W;
-  const place q = my_place(p, c0, 256);
+  constexpr int A = SAME ? 1 : 8;
+  __shared__ sum2<double> val[256 * A];
+  const int tid = threadIdx.x, item = blockIdx.z, slice = blockIdx.x, c0 = blockIdx.y * p.W;
+  const place<SAME> q = my_place<SAME>(p, c0, 256);
   const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
   const T* x = (const T*)p.x + (int64_t)item * p.P * p.C + q.c;
-  constexpr int A = SAME ? 1 : 8;
-  double s[A], ss[A];
+  sum2<double> s[A]{};
+  auto take = [&](const raw8<T>& d) {
 #pragma unroll
-  for (int i = 0; i < A; ++i) s[i] = 0.0, ss[i] = 0.0;
+    for (int i = 0; i < 8; ++i) {
+      const double v = (double)d[i];
+      s[SAME ? 0 : i].a += v;
+      s[SAME ? 0 : i].b = fma(v, v, s[SAME ? 0 : i].b);
+    }
+  };
   if (q.n > 0) {
     int r = r0 + q.r;
     for (; r + 3 * q.rpp < r1; r += 4 * q.rpp) {
@@ -292,54 +344,31 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(gn_args p) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) d[k] = load_raw<VEC>(x + (int64_t)(r + k * q.rpp) * p.C, q.n);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const double v = (double)(float)d[k].v[i];
-          s[SAME ? 0 : i] += v;
-          ss[SAME ? 0 : i] = fma(v, v, ss[SAME ? 0 : i]);
-        }
+      for (int k = 0; k < 4; ++k) take(d[k]);
     }
-    for (; r < r1; r += q.rpp) {
-      const raw8<T> d = load_raw<VEC>(x + (int64_t)r * p.C, q.n);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const double v = (double)(float)d.v[i];
-        s[SAME ? 0 : i] += v;
-        ss[SAME ? 0 : i] = fma(v, v, ss[SAME ? 0 : i]);
-      }
-    }
+    for (; r < r1; r += q.rpp) take(load_raw<VEC>(x + (int64_t)r * p.C, q.n));
   }
 #pragma unroll
-  for (int i = 0; i < A; ++i) val[tid * A + i] = make_double2(s[i], ss[i]);
+  for (int i = 0; i < A; ++i) val[tid * A + i] = s[i];
   __syncthreads();
-  double2* out = (double2*)p.part + ((int64_t)item * (p.slices * gridDim.y) + (int64_t)blockIdx.y * p.slices + slice) * p.G;
-  const int cend = min(c0 + p.W, p.C);
-  for (int g = wave; g < p.G; g += 4) {
-    const int lo = max(g * p.cg, c0), hi = min((g + 1) * p.cg, cend);   // (lo >= hi: outside this block)
-    double a = 0.0, b = 0.0;
-    if (lo < hi) {
-      const int w = SAME ? (hi - lo) >> 3 : hi - lo, base = SAME ? (lo - c0) >> 3 : lo - c0, pitch = SAME ? p.tpr : p.tpr * 8;
-      for (int e = lane; e < q.rpp * w; e += 64) {
-        const double2 v = val[(e / w) * pitch + base + e % w];
-        a += v.x;
-        b += v.y;
-      }
-      a = pgv_wave_sum_d(a);
-      b = pgv_wave_sum_d(b);
-    }
-    if (lane == 0) out[g] = make_double2(a, b);
-  }
+  sum2<double>* out = (sum2<double>*)p.part + ((int64_t)item * (p.slices * gridDim.y) + (int64_t)blockIdx.y * p.slices + slice) * p.G;
+  const int cend = min(c0 + p.W, p.C), pitch = SAME ? p.tpr : p.tpr * 8;
+  sum_groups<sum2<double>>(p.G, 256,
+      [&](int g, int e) {
+        const int lo = max(g * p.cg, c0), w = (min((g + 1) * p.cg, cend) - lo) / (SAME ? 8 : 1), r = e / w;
+        return val[r * pitch + (lo - c0) / (SAME ? 8 : 1) + (e - r * w)];
+      },
+      [&](int g) { return q.rpp * (max(0, min((g + 1) * p.cg, cend) - max(g * p.cg, c0)) / (SAME ? 8 : 1)); },
+      [&](int g, const sum2<double>& v) { out[g] = v; });
 }
 
 __global__ __launch_bounds__(64) void gn_finalize_kernel(gn_args p, int parts) {
   const int g = blockIdx.x, item = blockIdx.y, lane = threadIdx.x;
-  const double2* in = (const double2*)p.part + (int64_t)item * parts * p.G + g;
+  const sum2<double>* in = (const sum2<double>*)p.part + (int64_t)item * parts * p.G + g;
   double a = 0.0, b = 0.0;
   for (int e = lane; e < parts; e += 64) {
-    const double2 v = in[(int64_t)e * p.G];
-    a += v.x;
-    b += v.y;
+    a += in[(int64_t)e * p.G].a;
+    b += in[(int64_t)e * p.G].b;
   }
   a = pgv_wave_sum_d(a);
   b = pgv_wave_sum_d(b);
@@ -350,92 +379,118 @@ __global__ __launch_bounds__(64) void gn_finalize_kernel(gn_args p, int parts) {
   }
 }
 
-template <typename T, bool VEC, bool Q, int FMT>
+template <typename T, bool VEC, bool Q, int FMT, bool SAME>
 __global__ __launch_bounds__(256) void gn_apply_kernel(gn_args p) {
   const int item = blockIdx.z, slice = blockIdx.x, c0 = blockIdx.y * p.W;
-  const place q = my_place(p, c0, 256);
+  const place<SAME> q = my_place<SAME>(p, c0, 256);
   if (q.r >= q.rpp || (!Q && q.n == 0)) return;
   const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
   const T* x = (const T*)p.x + (int64_t)item * p.P * p.C + q.c;
-  chan ch;
+  chan<SAME> ch;
   load_affine(p, q, ch);
   load_stats(p, q, item, ch);
-  int r = r0 + q.r;
-  for (; r + 3 * q.rpp < r1; r += 4 * q.rpp) {
-    raw8<T> d[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (!Q || q.n > 0)
-        d[k] = load_raw<VEC>(x + (int64_t)(r + k * q.rpp) * p.C, q.n);
-      else
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[k].v[i] = (T)0.f;
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) put<VEC, Q, FMT>(p, q, ch, (int64_t)item * p.P + r + k * q.rpp, d[k]);
-  }
-  for (; r < r1; r += q.rpp) {
+  auto get = [&](int r) {
     raw8<T> d;
     if (!Q || q.n > 0)
       d = load_raw<VEC>(x + (int64_t)r * p.C, q.n);
     else
+      d.clear();
+    return d;
+  };
+  int r = r0 + q.r;
+  for (; r + 3 * q.rpp < r1; r += 4 * q.rpp) {
+    raw8<T> d[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d.v[i] = (T)0.f;
-    put<VEC, Q, FMT>(p, q, ch, (int64_t)item * p.P + r, d);
+    for (int k = 0; k < 4; ++k) d[k] = get(r + k * q.rpp);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) put<VEC, Q, FMT>(p, q, ch, (int64_t)item * p.P + r + k * q.rpp, d[k]);
   }
+  for (; r < r1; r += q.rpp) put<VEC, Q, FMT>(p, q, ch, (int64_t)item * p.P + r, get(r));
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
 // xh and du of 8 values
-template <typename T>
-__device__ __forceinline__ void grads8(const gn_args& p, const chan& k, const raw8<T>& x, const raw8<T>& gy, float (&xh)[8],
+template <bool SAME, typename T>
+__device__ __forceinline__ void grads8(const gn_args& p, const chan<SAME>& k, const raw8<T>& x, const raw8<T>& gy, float (&xh)[8],
                                        float (&du)[8]) {
   float u[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    xh[i] = ((float)x.v[i] - k.mu[i]) * k.rs[i];
+    xh[i] = (x[i] - k.mu[SAME ? 0 : i]) * k.rs[SAME ? 0 : i];
     u[i] = fmaf(xh[i], k.ga[i], k.be[i]);
-    du[i] = (float)gy.v[i];
+    du[i] = gy[i];
   }
   act_grad8(du, u, p.act, p.slope);
 }
-template <bool VEC, typename T>
-__device__ __forceinline__ void put_gx(const gn_args& p, const place& q, const chan& k, const float (&c1)[8], const float (&c2)[8],
-                                       int64_t pix, const raw8<T>& x, const raw8<T>& gy) {
+template <bool VEC, bool SAME, typename T>
+__device__ __forceinline__ void put_gx(const gn_args& p, const place<SAME>& q, const chan<SAME>& k, const float (&c1)[SAME ? 1 : 8],
+                                       const float (&c2)[SAME ? 1 : 8], int64_t pix, const raw8<T>& x, const raw8<T>& gy) {
   float xh[8], du[8], o[8];
   grads8(p, k, x, gy, xh, du);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = k.rs[i] * (fmaf(k.ga[i], du[i], -c1[i]) - xh[i] * c2[i]);
+  for (int i = 0; i < 8; ++i) {
+    const int h = SAME ? 0 : i;
+    o[i] = k.rs[h] * (fmaf(k.ga[i], du[i], -c1[h]) - xh[i] * c2[h]);
+  }
   store8<VEC>((T*)p.gx + pix * p.C + q.c, q.n, o);
 }
-// per-channel sums over the pixel phases of a workgroup: a = sum du, b = sum du xh -> tot[2][W]
+
+// Per-channel sums over the pixel phases of a workgroup, a = sum du and b = sum du xh, into tot[2][width]: the threads' values
+// go to val[2][NT * 8], every thread adds a share of the rows of one channel, the shares (in place) are added last.
 template <int NT>
-__device__ __forceinline__ void channel_sums(const gn_args& p, const place& q, const float (&a)[8], const float (&b)[8],
-                                             float* val /* [NT * 8] */, float* tot /* [2][NT * 8 at most] */, int width) {
+__device__ __forceinline__ void channel_sums(const gn_args& p, int n, int rpp, const float (&a)[8], const float (&b)[8], float* val,
+                                             float* tot, int width) {
+  f32x4* v = reinterpret_cast<f32x4*>(val + threadIdx.x * 8);
+  f32x4* w = reinterpret_cast<f32x4*>(val + NT * 8 + threadIdx.x * 8);
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    if (t) __syncthreads();
+  for (int h = 0; h < 2; ++h) {
+    f32x4 ta, tb;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) val[threadIdx.x * 8 + i] = i < q.n ? (t ? b[i] : a[i]) : 0.f;
-    __syncthreads();
+    for (int i = 0; i < 4; ++i) ta[i] = 4 * h + i < n ? a[4 * h + i] : 0.f, tb[i] = 4 * h + i < n ? b[4 * h + i] : 0.f;
+    v[h] = ta;
+    w[h] = tb;
+  }
+  __syncthreads();
+  const int shares = max(1, NT / width), pitch = p.tpr * 8;
+  if (shares == 1) {
     for (int c = threadIdx.x; c < width; c += NT) {
-      float s = 0.f;
-      for (int r = 0; r < q.rpp; ++r) s += val[r * p.tpr * 8 + c];
-      tot[t * width + c] = s;
+      float s = 0.f, t = 0.f;
+      for (int r = 0; r < rpp; ++r) s += val[r * pitch + c], t += val[NT * 8 + r * pitch + c];
+      tot[c] = s;
+      tot[width + c] = t;
+    }
+  } else {
+    const int sh = threadIdx.x / width, c = threadIdx.x - sh * width;
+    float s = 0.f, t = 0.f;
+    if (sh < shares)
+      for (int r = sh; r < rpp; r += shares) s += val[r * pitch + c], t += val[NT * 8 + r * pitch + c];
+    __syncthreads();
+    if (sh < shares) val[sh * width + c] = s, val[NT * 8 + sh * width + c] = t;
+    __syncthreads();
+    if (threadIdx.x < 2 * width && 2 * width <= NT) {   // both sums at once where the threads suffice
+      const int k = threadIdx.x / width, cc = threadIdx.x - k * width;
+      float u = 0.f;
+      for (int i = 0; i < shares; ++i) u += val[k * NT * 8 + i * width + cc];
+      tot[threadIdx.x] = u;
+    } else if (2 * width > NT && threadIdx.x < width) {
+      float u = 0.f, y = 0.f;
+      for (int i = 0; i < shares; ++i) u += val[i * width + threadIdx.x], y += val[NT * 8 + i * width + threadIdx.x];
+      tot[threadIdx.x] = u;
+      tot[width + threadIdx.x] = y;
     }
   }
   __syncthreads();
 }
 
 // fused: part [N][2][C] = the item's channel sums
-template <typename T, int NT, int KV, bool VEC>
+template <typename T, int NT, int KV, bool VEC, bool SAME>
 __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(gn_args p) {
-  extern __shared__ float sm[];
-  float* val = sm;                 // [NT * 8]
-  float* tot = sm + NT * 8;        // [2][width]
+  extern __shared__ __attribute__((aligned(16))) float sm[];
+  float* val = sm;                 // [2][NT * 8]
+  float* tot = sm + NT * 16;       // [2][width]
   __shared__ float gs[2][MAXG];
   const int item = blockIdx.y, c0 = blockIdx.x * p.W, width = min(p.W, p.C - c0);
-  const place q = my_place(p, c0, NT);
+  const place<SAME> q = my_place<SAME>(p, c0, NT);
   const T* x = (const T*)p.x + (int64_t)item * p.P * p.C;
   const T* gy = (const T*)p.gy + (int64_t)item * p.P * p.C;
   raw8<T> d[KV], e[KV];
@@ -446,11 +501,11 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(gn_args p) {
       d[k] = load_raw<VEC>(x + (int64_t)r * p.C + q.c, q.n);
       e[k] = load_raw<VEC>(gy + (int64_t)r * p.C + q.c, q.n);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) d[k].v[i] = (T)0.f, e[k].v[i] = (T)0.f;
+      d[k].clear();
+      e[k].clear();
     }
   }
-  chan ch;
+  chan<SAME> ch;
   load_affine(p, q, ch);
   load_stats(p, q, item, ch);
   float a[8], b[8];
@@ -464,21 +519,20 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(gn_args p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) a[i] += du[i], b[i] = fmaf(du[i], xh[i], b[i]);
     }
-  channel_sums<NT>(p, q, a, b, val, tot, width);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int g = wave; g < width / p.cg; g += NT / 64) {
-    float s1 = 0.f, s2 = 0.f;
-    for (int i = lane; i < p.cg; i += 64) {
-      const int c = g * p.cg + i;
-      const float ga = p.gamma ? p.gamma[c0 + c] : 1.f;
-      s1 = fmaf(ga, tot[c], s1);
-      s2 = fmaf(ga, tot[width + c], s2);
-    }
-    s1 = pgv_wave_sum(s1);
-    s2 = pgv_wave_sum(s2);
-    const float n = (float)p.P * (float)p.cg;
-    if (lane == 0) gs[0][g] = s1 / n, gs[1][g] = s2 / n;
-  }
+#pragma unroll
+  for (int k = 0; k < KV; ++k) d[k].forget(), e[k].forget();
+  channel_sums<NT>(p, q.n, q.rpp, a, b, val, tot, width);
+  const float inv_n = 1.f / ((float)p.P * (float)p.cg);
+  sum_groups<sum2<float>>(width / p.cg, NT,
+      [&](int g, int i) {
+        const int c = g * p.cg + i;
+        const float ga = p.gamma ? p.gamma[c0 + c] : 1.f;
+        sum2<float> v;
+        v.a = ga * tot[c];
+        v.b = ga * tot[width + c];
+        return v;
+      },
+      [&](int) { return p.cg; }, [&](int g, const sum2<float>& v) { gs[0][g] = v.a * inv_n, gs[1][g] = v.b * inv_n; });
   if (p.part)
     for (int c = threadIdx.x; c < width; c += NT) {
       p.part[((int64_t)item * 2) * p.C + c0 + c] = tot[c];
@@ -486,10 +540,10 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(gn_args p) {
     }
   __syncthreads();
   if (q.n == 0) return;
-  float c1[8], c2[8];
+  float c1[q.A], c2[q.A];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int g = i < q.n ? (q.c + i - c0) / p.cg : 0;
+  for (int i = 0; i < q.A; ++i) {
+    const int g = i < q.n ? q.g[i] - c0 / p.cg : 0;
     c1[i] = gs[0][g];
     c2[i] = gs[1][g];
   }
@@ -501,31 +555,43 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(gn_args p) {
 }
 
 // two-pass, first: part [N][slices][2][C]
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool SAME>
 __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(gn_args p) {
-  __shared__ float val[2048], tot[4096];
+  __shared__ __attribute__((aligned(16))) float val[4096];
+  __shared__ float tot[4096];
   const int item = blockIdx.z, slice = blockIdx.x, c0 = blockIdx.y * p.W, width = min(p.W, p.C - c0);
-  const place q = my_place(p, c0, 256);
+  const place<SAME> q = my_place<SAME>(p, c0, 256);
   const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
   const int64_t base = (int64_t)item * p.P * p.C + q.c;
   const T* x = (const T*)p.x + base;
   const T* gy = (const T*)p.gy + base;
-  chan ch;
+  chan<SAME> ch;
   load_affine(p, q, ch);
   load_stats(p, q, item, ch);
   float a[8], b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) a[i] = 0.f, b[i] = 0.f;
-  if (q.n > 0)
-#pragma unroll 2
-    for (int r = r0 + q.r; r < r1; r += q.rpp) {
-      const raw8<T> d = load_raw<VEC>(x + (int64_t)r * p.C, q.n), e = load_raw<VEC>(gy + (int64_t)r * p.C, q.n);
-      float xh[8], du[8];
-      grads8(p, ch, d, e, xh, du);
+  auto take = [&](const raw8<T>& d, const raw8<T>& e) {
+    float xh[8], du[8];
+    grads8(p, ch, d, e, xh, du);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] += du[i], b[i] = fmaf(du[i], xh[i], b[i]);
+    for (int i = 0; i < 8; ++i) a[i] += du[i], b[i] = fmaf(du[i], xh[i], b[i]);
+  };
+  if (q.n > 0) {
+    int r = r0 + q.r;
+    for (; r + 3 * q.rpp < r1; r += 4 * q.rpp) {
+      raw8<T> d[4], e[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        d[k] = load_raw<VEC>(x + (int64_t)(r + k * q.rpp) * p.C, q.n);
+        e[k] = load_raw<VEC>(gy + (int64_t)(r + k * q.rpp) * p.C, q.n);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) take(d[k], e[k]);
     }
-  channel_sums<256>(p, q, a, b, val, tot, width);
+    for (; r < r1; r += q.rpp) take(load_raw<VEC>(x + (int64_t)r * p.C, q.n), load_raw<VEC>(gy + (int64_t)r * p.C, q.n));
+  }
+  channel_sums<256>(p, q.n, q.rpp, a, b, val, tot, width);
   float* out = p.part + ((int64_t)item * p.slices + slice) * 2 * p.C + c0;
   for (int c = threadIdx.x; c < width; c += 256) {
     out[c] = tot[c];
@@ -533,16 +599,36 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(gn_args p) {
   }
 }
 
-// slices -> the group means of h and h xh
-__global__ __launch_bounds__(64) void gn_bwd_finalize_kernel(gn_args p) {
+// slices -> channel sums of the item, item_tot [N][2][C]: 32 channels x 8 interleaved chains of slices per workgroup
+__global__ __launch_bounds__(256) void gn_bwd_item_kernel(gn_args p, float* __restrict__ item_tot) {
+  __shared__ float red[8][64];
+  const int l = threadIdx.x & 31, ph = threadIdx.x >> 5, c = blockIdx.x * 32 + l, item = blockIdx.y;
+  const float* in = p.part + (int64_t)item * p.slices * 2 * p.C + c;
+  float a = 0.f, b = 0.f;
+  if (c < p.C)
+#pragma unroll 4
+    for (int r = ph; r < p.slices; r += 8) {
+      a += in[(int64_t)r * 2 * p.C];
+      b += in[((int64_t)r * 2 + 1) * p.C];
+    }
+  red[ph][l] = a;
+  red[ph][32 + l] = b;
+  __syncthreads();
+  if (threadIdx.x < 64 && c < p.C) {
+    float s = 0.f;
+    for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
+    item_tot[((int64_t)item * 2 + (threadIdx.x >> 5)) * p.C + c] = s;
+  }
+}
+// channel sums -> the group means of h and h xh: one wave per (group, item)
+__global__ __launch_bounds__(64) void gn_bwd_coef_kernel(gn_args p, const float* __restrict__ item_tot) {
   const int g = blockIdx.x, item = blockIdx.y, lane = threadIdx.x;
-  const float* in = p.part + (int64_t)item * p.slices * 2 * p.C + g * p.cg;
+  const float* in = item_tot + (int64_t)item * 2 * p.C + g * p.cg;
   double s1 = 0.0, s2 = 0.0;
-  for (int64_t e = lane; e < (int64_t)p.slices * p.cg; e += 64) {
-    const int sl = (int)(e / p.cg), c = (int)(e % p.cg);
+  for (int c = lane; c < p.cg; c += 64) {
     const double ga = p.gamma ? (double)p.gamma[g * p.cg + c] : 1.0;
-    s1 += ga * (double)in[(int64_t)sl * 2 * p.C + c];
-    s2 += ga * (double)in[(int64_t)sl * 2 * p.C + p.C + c];
+    s1 += ga * (double)in[c];
+    s2 += ga * (double)in[p.C + c];
   }
   s1 = pgv_wave_sum_d(s1);
   s2 = pgv_wave_sum_d(s2);
@@ -553,22 +639,22 @@ __global__ __launch_bounds__(64) void gn_bwd_finalize_kernel(gn_args p) {
   }
 }
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool SAME>
 __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(gn_args p) {
   const int item = blockIdx.z, slice = blockIdx.x, c0 = blockIdx.y * p.W;
-  const place q = my_place(p, c0, 256);
+  const place<SAME> q = my_place<SAME>(p, c0, 256);
   if (q.n == 0) return;
   const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
   const int64_t base = (int64_t)item * p.P * p.C + q.c;
   const T* x = (const T*)p.x + base;
   const T* gy = (const T*)p.gy + base;
-  chan ch;
+  chan<SAME> ch;
   load_affine(p, q, ch);
   load_stats(p, q, item, ch);
-  float c1[8], c2[8];
+  float c1[q.A], c2[q.A];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t g = (int64_t)item * p.G + (i < q.n ? (q.c + i) / p.cg : 0);
+  for (int i = 0; i < q.A; ++i) {
+    const int64_t g = (int64_t)item * p.G + q.g[i];
     c1[i] = p.coef[2 * g];
     c2[i] = p.coef[2 * g + 1];
   }
@@ -586,7 +672,7 @@ __global__ __launch_bounds__(256) void gn_param_grads_kernel(const float* __rest
   const int l = threadIdx.x & 31, ph = threadIdx.x >> 5, c = blockIdx.x * 32 + l;
   double a = 0.0, b = 0.0;
   if (c < C)
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t r = ph; r < rows; r += 8) {
       a += (double)part[r * 2 * C + c];
       b += (double)part[(r * 2 + 1) * C + c];
@@ -632,10 +718,14 @@ gn_plan make_gn_plan(int64_t N, int64_t P, int64_t C, int64_t G, int esize, int 
   int64_t tpr = pgv_cdiv(W, 8);
   if (kind == 1) tpr = pgv_cdiv(W, F8B) * 16;
   const int64_t groups = pgv_cdiv(W, cg);
-  static const int cfg[][2] = {{256, 1}, {256, 4}, {1024, 4}, {1024, 8}};
+  // {threads, pieces of 8 values a thread holds, bytes per value at most}: the pieces take 8 or 4 registers each, twice that for
+  // the backward pass, out of 128 with 1024 threads and 512 with 256
+  static const int fwd[][3] = {{256, 1, 4}, {256, 4, 4}, {256, 8, 4}, {1024, 4, 4}, {1024, 8, 4}, {1024, 16, 2}, {1024, 24, 2}};
+  static const int bwd[][3] = {{256, 1, 4}, {256, 4, 4}, {256, 8, 4}, {1024, 4, 4}, {1024, 8, 2}};
   if (groups <= MAXG)
-    for (const auto& c : cfg) {
-      if (kind == 2 && c[1] == 8) break;   // x and gy: twice the registers
+    for (int i = 0; i < (kind == 2 ? 5 : 7); ++i) {
+      const int* c = kind == 2 ? bwd[i] : fwd[i];
+      if (esize > c[2]) continue;
       const int64_t rpp = c[0] / tpr;
       if (rpp >= 1 && P <= rpp * c[1]) {
         r.fused = true;
@@ -668,66 +758,73 @@ int gn_check(const char* who, int64_t N, int64_t P, int64_t C, int64_t G, int dt
   return PGV_OK;
 }
 
-template <typename T, bool VEC, bool Q, int FMT>
+template <typename T, bool VEC, bool Q, int FMT, bool SAME>
 int gn_forward(gn_args p, const gn_plan& pl, hipStream_t st) {
-  const bool same = p.cg % 8 == 0;
   p.W = pl.W;
   p.tpr = pl.tpr;
   p.slices = pl.slices;
   if (pl.fused) {
     const dim3 grid((unsigned)pl.colblocks, (unsigned)p.N);
-#define PGV_F(NT, KV)                                                            \
-  same ? gn_fwd_fused_kernel<T, NT, KV, VEC, Q, FMT, true><<<grid, NT, 0, st>>>(p) \
-       : gn_fwd_fused_kernel<T, NT, KV, VEC, Q, FMT, false><<<grid, NT, 0, st>>>(p)
+#define PGV_F(NT, KV) gn_fwd_fused_kernel<T, NT, KV, VEC, Q, FMT, SAME><<<grid, NT, 0, st>>>(p)
     if (pl.nt == 256)
-      pl.kv == 1 ? (PGV_F(256, 1)) : (PGV_F(256, 4));
-    else
-      pl.kv == 4 ? (PGV_F(1024, 4)) : (PGV_F(1024, 8));
+      pl.kv == 1 ? PGV_F(256, 1) : pl.kv == 4 ? PGV_F(256, 4) : PGV_F(256, 8);
+    else if (pl.kv <= 8)
+      pl.kv == 4 ? PGV_F(1024, 4) : PGV_F(1024, 8);
+    else if constexpr (sizeof(T) == 2)
+      pl.kv == 16 ? PGV_F(1024, 16) : PGV_F(1024, 24);
 #undef PGV_F
     return PGV_OK;
   }
   const dim3 grid((unsigned)pl.slices, (unsigned)pl.colblocks, (unsigned)p.N);
-  if (same)
-    gn_stats_kernel<T, VEC, true><<<grid, 256, 0, st>>>(p);
-  else
-    gn_stats_kernel<T, VEC, false><<<grid, 256, 0, st>>>(p);
+  gn_stats_kernel<T, VEC, SAME><<<grid, 256, 0, st>>>(p);
   gn_finalize_kernel<<<dim3((unsigned)p.G, (unsigned)p.N), 64, 0, st>>>(p, pl.slices * pl.colblocks);
-  gn_apply_kernel<T, VEC, Q, FMT><<<grid, 256, 0, st>>>(p);
+  gn_apply_kernel<T, VEC, Q, FMT, SAME><<<grid, 256, 0, st>>>(p);
   return PGV_OK;
 }
 
-template <typename T, int NT, int KV, bool VEC>
+template <typename T, int NT, int KV, bool VEC, bool SAME>
 int launch_bwd_fused(const gn_args& p, dim3 grid, hipStream_t st) {
-  auto k = gn_bwd_fused_kernel<T, NT, KV, VEC>;
-  constexpr int most = 3 * NT * 8 * (int)sizeof(float);   // W is at most 8 NT channels
+  auto k = gn_bwd_fused_kernel<T, NT, KV, VEC, SAME>;
+  constexpr int most = NT * 16 * (int)sizeof(float) + 2 * 8 * NT * (int)sizeof(float);   // W is at most 8 NT channels
   static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, most);
   if (once != hipSuccess) {
     pgv_set_error("pgv_group_norm_act_bwd: %d bytes of LDS refused: %s", most, hipGetErrorString(once));
     return PGV_E_LAUNCH;
   }
-  k<<<grid, NT, sizeof(float) * ((size_t)NT * 8 + 2 * (size_t)p.W), st>>>(p);
+  k<<<grid, NT, sizeof(float) * ((size_t)NT * 16 + 2 * (size_t)p.W), st>>>(p);
   return PGV_OK;
 }
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool SAME>
 int gn_backward(gn_args p, const gn_plan& pl, float* ggamma, float* gbeta, hipStream_t st) {
   p.W = pl.W;
   p.tpr = pl.tpr;
-  p.slices = pl.fused ? 1 : pl.slices;
+  p.slices = pl.slices;
+  const float* item_tot = p.part;
   if (pl.fused) {
     const dim3 grid((unsigned)pl.colblocks, (unsigned)p.N);
-    const int rc = pl.nt == 1024 ? launch_bwd_fused<T, 1024, 4, VEC>(p, grid, st)
-                   : pl.kv == 4  ? launch_bwd_fused<T, 256, 4, VEC>(p, grid, st)
-                                 : launch_bwd_fused<T, 256, 1, VEC>(p, grid, st);
+    int rc = PGV_OK;
+    if (pl.nt == 256)
+      rc = pl.kv == 1   ? launch_bwd_fused<T, 256, 1, VEC, SAME>(p, grid, st)
+           : pl.kv == 4 ? launch_bwd_fused<T, 256, 4, VEC, SAME>(p, grid, st)
+                        : launch_bwd_fused<T, 256, 8, VEC, SAME>(p, grid, st);
+    else if (pl.kv == 4)
+      rc = launch_bwd_fused<T, 1024, 4, VEC, SAME>(p, grid, st);
+    else if constexpr (sizeof(T) == 2)
+      rc = launch_bwd_fused<T, 1024, 8, VEC, SAME>(p, grid, st);
     if (rc != PGV_OK) return rc;
   } else {
     const dim3 grid((unsigned)pl.slices, (unsigned)pl.colblocks, (unsigned)p.N);
-    gn_bwd_sums_kernel<T, VEC><<<grid, 256, 0, st>>>(p);
-    gn_bwd_finalize_kernel<<<dim3((unsigned)p.G, (unsigned)p.N), 64, 0, st>>>(p);
-    gn_bwd_apply_kernel<T, VEC><<<grid, 256, 0, st>>>(p);
+    float* tot = p.part + (int64_t)p.N * pl.slices * 2 * p.C;
+    p.coef = tot + (int64_t)p.N * 2 * p.C;
+    gn_bwd_sums_kernel<T, VEC, SAME><<<grid, 256, 0, st>>>(p);
+    gn_bwd_item_kernel<<<dim3((unsigned)pgv_cdiv(p.C, 32), (unsigned)p.N), 256, 0, st>>>(p, tot);
+    gn_bwd_coef_kernel<<<dim3((unsigned)p.G, (unsigned)p.N), 64, 0, st>>>(p, tot);
+    gn_bwd_apply_kernel<T, VEC, SAME><<<grid, 256, 0, st>>>(p);
+    item_tot = tot;
   }
   if (ggamma || gbeta)
-    gn_param_grads_kernel<<<dim3((unsigned)pgv_cdiv(p.C, 32)), 256, 0, st>>>(p.part, (int64_t)p.N * p.slices, p.C, ggamma, gbeta);
+    gn_param_grads_kernel<<<dim3((unsigned)pgv_cdiv(p.C, 32)), 256, 0, st>>>(item_tot, p.N, p.C, ggamma, gbeta);
   return PGV_OK;
 }
 
@@ -736,7 +833,7 @@ int gn_backward(gn_args p, const gn_plan& pl, float* ggamma, float* gbeta, hipSt
 extern "C" int64_t pgv_group_norm_workspace(int64_t N, int64_t P, int64_t C, int64_t G, int dtype, int kind) {
   if (N <= 0 || P <= 0 || C <= 0 || G <= 0 || C % G || !f8_dt_ok(dtype) || kind < 0 || kind > 2) return 0;
   const gn_plan pl = make_gn_plan(N, P, C, G, f8_dt_size(dtype), kind);
-  if (kind == 2) return 4 * (pl.fused ? N * 2 * C : N * pl.slices * 2 * C + N * G * 2);
+  if (kind == 2) return 4 * (pl.fused ? N * 2 * C : N * (pl.slices + 1) * 2 * C + N * G * 2);
   const int64_t stats = kind == 1 && !pl.fused ? 8 * N * G : 0;   // mean and rstd live here when the caller has no use for them
   return stats + (pl.fused ? 0 : 16 * N * G * pl.slices * pl.colblocks);
 }
@@ -769,7 +866,11 @@ static int gn_fwd_any(const char* who, const void* x, int dtype, int64_t N, int6
   const bool vec = C % 8 == 0 && (uintptr_t)x % 16 == 0 && (q || (uintptr_t)y % 16 == 0);
   hipStream_t st = pgv_stream(stream);
   int r;
-#define PGV_T(T, Q, FMT) (vec ? gn_forward<T, true, Q, FMT>(p, pl, st) : gn_forward<T, false, Q, FMT>(p, pl, st))
+  // (C/G a multiple of 8 makes C one: rows that are not 16-byte pieces then come from an unaligned base alone)
+  const bool same = p.cg % 8 == 0;
+#define PGV_T(T, Q, FMT)                                                                                    \
+  (vec ? (same ? gn_forward<T, true, Q, FMT, true>(p, pl, st) : gn_forward<T, true, Q, FMT, false>(p, pl, st)) \
+       : gn_forward<T, false, Q, FMT, false>(p, pl, st))
 #define PGV_D(Q, FMT) (dtype == PGV_DT_F32 ? PGV_T(float, Q, FMT) : dtype == PGV_DT_BF16 ? PGV_T(__bf16, Q, FMT) : PGV_T(_Float16, Q, FMT))
   if (!q)
     r = PGV_D(false, PGV_F8_E4M3);
@@ -818,10 +919,12 @@ extern "C" int pgv_group_norm_act_bwd(const void* gy, const void* x, int dtype, 
   p.x = x, p.gy = gy, p.gx = gx, p.gamma = gamma, p.beta = beta, p.slope = slope, p.act = act;
   p.mean = const_cast<float*>(mean), p.rstd = const_cast<float*>(rstd);
   p.part = (float*)workspace;
-  p.coef = pl.fused ? nullptr : p.part + N * pl.slices * 2 * C;
   const bool vec = C % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)gy % 16 == 0 && (uintptr_t)gx % 16 == 0;
   hipStream_t st = pgv_stream(stream);
-#define PGV_T(T) (vec ? gn_backward<T, true>(p, pl, ggamma, gbeta, st) : gn_backward<T, false>(p, pl, ggamma, gbeta, st))
+  const bool same = p.cg % 8 == 0;
+#define PGV_T(T)                                                                                                  \
+  (vec ? (same ? gn_backward<T, true, true>(p, pl, ggamma, gbeta, st) : gn_backward<T, true, false>(p, pl, ggamma, gbeta, st)) \
+       : gn_backward<T, false, false>(p, pl, ggamma, gbeta, st))
   const int r = dtype == PGV_DT_F32 ? PGV_T(float) : dtype == PGV_DT_BF16 ? PGV_T(__bf16) : PGV_T(_Float16);
 #undef PGV_T
   if (r != PGV_OK) return r;

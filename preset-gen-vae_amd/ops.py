@@ -885,7 +885,6 @@ F8_FORMATS = {'e4m3': (0, torch.float8_e4m3fn), 'e5m2': (1, torch.float8_e5m2)}
 F8_BLOCK_KINDS = {'row': 0, 'tile': 1}
 _F8_CODE = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 _DT_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_F8_EMPTY_SCALE = {'row': lambda r, kb: (kb, r), 'tile': lambda r, kb: (-(-r // 128), kb)}
 
 
 class Fp8Blocks(NamedTuple):
@@ -904,26 +903,18 @@ class Fp8Blocks(NamedTuple):
         return (self.q.float().view(R, -1, 128) * s.unsqueeze(-1)).view(R, -1)[:, :self.cols]
 
 
-class _on_device:
-    """Makes the device of ``t`` current for a call (a no-op in the usual case) and gives its stream."""
-    __slots__ = ('guard', 'device')
+# (the accessors behind torch.cuda.current_device / current_stream: a call of a few microseconds has no room for their wrappers)
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
-    def __init__(self, t):
-        self.device = t.device
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _elsewhere(t, fn, *args):
+    """``fn(*args)`` with the device of ``t`` current."""
+    with torch.cuda.device(t.device):
+        return fn(*args)
 
 
 def _values(who, t, ndim=2):
-    """(element type code) of a value tensor; raises on anything the kernels do not read."""
+    """Element type code of a value tensor; raises on anything the kernels do not read."""
     if not t.is_cuda:
         raise RuntimeError("preset-gen-vae_amd ops need tensors on a ROCm device (no CPU fallback exists)")
     code = _DT_CODE.get(t.dtype)
@@ -946,41 +937,42 @@ def _row_stride(who, t):
 
 
 def _same_device(who, t, *others):
+    index = t.get_device()
     for o in others:
-        if o is not None and o.device != t.device:
+        if o is not None and o.get_device() != index:
             raise RuntimeError(f"{who}: tensors on different devices ({t.device} and {o.device})")
 
 
 def _f32_vector(who, name, t, n):
-    if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != n):
+    if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous()):
         raise ValueError(f"{who}: {name} must be {n} contiguous float32 values")
 
 
-def _f8_alloc(R, C, block, fmt, device):
-    Kp = (C + 127) // 128 * 128
-    return Fp8Blocks(torch.empty((R, Kp), dtype=F8_FORMATS[fmt][1], device=device),
-                     torch.empty(_F8_EMPTY_SCALE[block](R, Kp // 128), dtype=torch.float32, device=device), block, C)
+def _f8_alloc(like, R, C, block, fmt):
+    Kb = (C + 127) // 128
+    return Fp8Blocks(like.new_empty((R, Kb * 128), dtype=F8_FORMATS[fmt][1]),
+                     like.new_empty((Kb, R) if block == 'row' else ((R + 127) // 128, Kb), dtype=torch.float32), block, C)
 
 
 def _f8_quantize(x, block, fmt, want, want_t, colsum=False):
     if block not in F8_BLOCK_KINDS or fmt not in F8_FORMATS:
         raise ValueError(f"fp8_quantize: block is 'row' or 'tile', fmt 'e4m3' or 'e5m2' (got {block!r}, {fmt!r})")
     code = _values("fp8_quantize", x)
+    if x.get_device() != _current_device():
+        return _elsewhere(x, _f8_quantize, x, block, fmt, want, want_t, colsum)
     ld = _row_stride("fp8_quantize", x)
     R, C = x.shape
-    dev = x.device
-    t = _f8_alloc(R, C, block, fmt, dev) if want else None
-    tt = _f8_alloc(C, R, block, fmt, dev) if want_t else None
-    cs = torch.empty(C, dtype=torch.float32, device=dev) if colsum else None
+    t = _f8_alloc(x, R, C, block, fmt) if want else None
+    tt = _f8_alloc(x, C, R, block, fmt) if want_t else None
+    cs = x.new_empty(C, dtype=torch.float32) if colsum else None
     if R == 0 or C == 0:
         return t, tt, cs.zero_() if colsum else None
-    ws = torch.empty((R + 127) // 128 * C, dtype=torch.float32, device=dev) if colsum else None
-    with _on_device(x) as stream:
-        _lib.check(_lib.load().pgv_f8_quantize(x.data_ptr(), code, R, C, ld, F8_BLOCK_KINDS[block], F8_FORMATS[fmt][0],
-                                               t.q.data_ptr() if want else None, t.scale.data_ptr() if want else None,
-                                               tt.q.data_ptr() if want_t else None, tt.scale.data_ptr() if want_t else None,
-                                               _p(cs), _p(ws), 0 if ws is None else ws.numel() * 4, stream),
-                   "pgv_f8_quantize")
+    ws = x.new_empty((R + 127) // 128 * C, dtype=torch.float32) if colsum else None
+    _lib.check(_lib.load().pgv_f8_quantize(x.data_ptr(), code, R, C, ld, F8_BLOCK_KINDS[block], F8_FORMATS[fmt][0],
+                                           t.q.data_ptr() if want else None, t.scale.data_ptr() if want else None,
+                                           tt.q.data_ptr() if want_t else None, tt.scale.data_ptr() if want_t else None,
+                                           _p(cs), _p(ws), 0 if ws is None else ws.numel() * 4, _raw_stream(x.get_device())),
+               "pgv_f8_quantize")
     return t, tt, cs
 
 
@@ -999,18 +991,20 @@ def _f8_operand(who, t):
     if not isinstance(t, Fp8Blocks):
         raise TypeError(f"{who}: expected Fp8Blocks (fp8_quantize), got {type(t).__name__}")
     q, s, block, cols = t
-    if not q.is_cuda or q.dtype not in _F8_CODE or q.dim() != 2 or not q.is_contiguous():
+    code = _F8_CODE.get(q.dtype)
+    if code is None or not q.is_cuda or q.dim() != 2 or not q.is_contiguous():
         raise RuntimeError(f"{who}: the bytes must be a contiguous 2-d float8 tensor on a ROCm device")
     if block not in F8_BLOCK_KINDS:
         raise ValueError(f"{who}: unknown block kind {block!r}")
     R, Kp = q.shape
-    if Kp != (cols + 127) // 128 * 128:
-        raise ValueError(f"{who}: {cols} columns take rows of {(cols + 127) // 128 * 128} bytes, got {Kp}")
-    _f32_vector(who, "scale", s, ((R if block == 'row' else (R + 127) // 128) * (Kp // 128)))
-    if tuple(s.shape) != _F8_EMPTY_SCALE[block](R, Kp // 128):
-        raise ValueError(f"{who}: scales of shape {tuple(s.shape)} do not belong to {block} blocks of {tuple(q.shape)}")
-    _same_device(who, q, s)
-    return _F8_CODE[q.dtype]
+    Kb = (cols + 127) // 128
+    if Kp != Kb * 128:
+        raise ValueError(f"{who}: {cols} columns take rows of {Kb * 128} bytes, got {Kp}")
+    if s.dtype != torch.float32 or s.shape != ((Kb, R) if block == 'row' else ((R + 127) // 128, Kb)) or not s.is_contiguous():
+        raise ValueError(f"{who}: scales of shape {tuple(s.shape)} ({s.dtype}) do not belong to {block} blocks of {tuple(q.shape)}")
+    if s.get_device() != q.get_device():
+        raise RuntimeError(f"{who}: tensors on different devices ({q.device} and {s.device})")
+    return code
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1023,13 +1017,13 @@ def _f8_fused(M, b_block):
     return bool(_lib.load().pgv_f8_linear_fused(M, b_block))
 
 
-def _f8_out(who, M, N, dtype, device, out):
+def _f8_out(who, like, M, N, dtype, out):
     if dtype not in _DT_CODE:
         raise ValueError(f"{who}: output type {dtype} is not float32, bfloat16 or float16")
     if out is None:
-        return torch.empty((M, N), dtype=dtype, device=device)
-    if out.device != device or out.dtype != dtype or tuple(out.shape) != (M, N) or not out.is_contiguous():
-        raise ValueError(f"{who}: out must be a contiguous {dtype} [{M}, {N}] tensor on {device}")
+        return like.new_empty((M, N), dtype=dtype)
+    if out.device != like.device or out.dtype != dtype or tuple(out.shape) != (M, N) or not out.is_contiguous():
+        raise ValueError(f"{who}: out must be a contiguous {dtype} [{M}, {N}] tensor on {like.device}")
     return out
 
 
@@ -1037,6 +1031,8 @@ def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16, out=None):
     """a [M, K] ('row' blocks, e4m3 or e5m2) times the transpose of b [N, K] ('row' or 'tile' blocks, e4m3), + ``bias`` [N]
     (float32): [M, N], summed in float32 and rounded once to ``out_dtype`` (``pgv_f8_matmul``)."""
     fmt = _f8_operand("fp8_matmul", a)
+    if a.q.get_device() != _current_device():
+        return _elsewhere(a.q, fp8_matmul, a, b, bias, out_dtype, out)
     if _f8_operand("fp8_matmul", b) != 0:
         raise ValueError("fp8_matmul: the second operand must be e4m3")
     if a.block != 'row':
@@ -1046,18 +1042,17 @@ def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16, out=None):
         raise ValueError(f"fp8_matmul: reductions of {K} and {b.cols} values")
     _f32_vector("fp8_matmul", "bias", bias, N)
     _same_device("fp8_matmul", a.q, b.q, bias)
-    y = _f8_out("fp8_matmul", M, N, out_dtype, a.q.device, out)
+    y = _f8_out("fp8_matmul", a.scale, M, N, out_dtype, out)
     if M == 0 or N == 0:
         return y
     if K == 0:
         return y.zero_() if bias is None else y.copy_(bias.expand(M, N))
     kind = F8_BLOCK_KINDS[b.block]
     nbytes = _f8_matmul_ws(M, N, K, kind)
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=y.device) if nbytes else None
-    with _on_device(y) as stream:
-        _lib.check(_lib.load().pgv_f8_matmul(M, N, K, a.q.data_ptr(), a.scale.data_ptr(), fmt, b.q.data_ptr(),
-                                             b.scale.data_ptr(), kind, _p(bias), y.data_ptr(), _DT_CODE[y.dtype], _p(ws),
-                                             nbytes, stream), "pgv_f8_matmul")
+    ws = y.new_empty(nbytes // 4, dtype=torch.float32) if nbytes else None
+    _lib.check(_lib.load().pgv_f8_matmul(M, N, K, a.q.data_ptr(), a.scale.data_ptr(), fmt, b.q.data_ptr(),
+                                         b.scale.data_ptr(), kind, _p(bias), y.data_ptr(), _DT_CODE[y.dtype], _p(ws),
+                                         nbytes, _raw_stream(y.get_device())), "pgv_f8_matmul")
     return y
 
 
@@ -1065,6 +1060,8 @@ def fp8_linear(x, w, bias=None, out_dtype=None, out=None):
     """nn.Linear on a weight that was quantised once (``w`` = ``fp8_quantize(weight, 'tile')``): y = Q(x) w^T + bias in the type
     of x (or ``out_dtype``), Q = 'row' blocks of e4m3 (``pgv_f8_linear``).  Few rows take one launch."""
     code = _values("fp8_linear", x)
+    if x.get_device() != _current_device():
+        return _elsewhere(x, fp8_linear, x, w, bias, out_dtype, out)
     ld = _row_stride("fp8_linear", x)
     if _f8_operand("fp8_linear", w) != 0:
         raise ValueError("fp8_linear: the weight must be e4m3")
@@ -1073,20 +1070,19 @@ def fp8_linear(x, w, bias=None, out_dtype=None, out=None):
         raise ValueError(f"fp8_linear: x has {K} features, the weight {w.cols}")
     _f32_vector("fp8_linear", "bias", bias, N)
     _same_device("fp8_linear", x, w.q, bias)
-    y = _f8_out("fp8_linear", M, N, x.dtype if out_dtype is None else out_dtype, x.device, out)
+    y = _f8_out("fp8_linear", x, M, N, x.dtype if out_dtype is None else out_dtype, out)
     if M == 0 or N == 0:
         return y
     if K == 0:
         return y.zero_() if bias is None else y.copy_(bias.expand(M, N))
     kind = F8_BLOCK_KINDS[w.block]
     nbytes = _f8_matmul_ws(M, N, K, kind)
-    xq = None if _f8_fused(M, kind) else _f8_alloc(M, K, 'row', 'e4m3', x.device)
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device) if nbytes else None
-    with _on_device(x) as stream:
-        _lib.check(_lib.load().pgv_f8_linear(x.data_ptr(), code, M, K, ld, w.q.data_ptr(), w.scale.data_ptr(), kind, N, _p(bias),
-                                             None if xq is None else xq.q.data_ptr(),
-                                             None if xq is None else xq.scale.data_ptr(), y.data_ptr(), _DT_CODE[y.dtype],
-                                             _p(ws), nbytes, stream), "pgv_f8_linear")
+    xq = None if _f8_fused(M, kind) else _f8_alloc(x, M, K, 'row', 'e4m3')
+    ws = x.new_empty(nbytes // 4, dtype=torch.float32) if nbytes else None
+    _lib.check(_lib.load().pgv_f8_linear(x.data_ptr(), code, M, K, ld, w.q.data_ptr(), w.scale.data_ptr(), kind, N, _p(bias),
+                                         None if xq is None else xq.q.data_ptr(),
+                                         None if xq is None else xq.scale.data_ptr(), y.data_ptr(), _DT_CODE[y.dtype],
+                                         _p(ws), nbytes, _raw_stream(x.get_device())), "pgv_f8_linear")
     return y
 
 
@@ -1162,19 +1158,17 @@ def group_norm_act_fwd(x, groups, weight=None, bias=None, eps=1e-5, act=PGV_ACT_
     format): (y, mean, rstd), y in the type of x, mean / rstd [items, groups] float32 for ``group_norm_act_bwd``
     (``pgv_group_norm_act_fwd``).  ``weight`` / ``bias``: float32 [channels] or None."""
     code, N, P, C = _gn_args("group_norm_act_fwd", x, groups, weight, bias, act)
+    if x.get_device() != _current_device():
+        return _elsewhere(x, group_norm_act_fwd, x, groups, weight, bias, eps, act, slope)
     y = torch.empty_like(x)
-    stats = torch.empty((2, N, groups), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
-    if x.numel() == 0:
-        if stats.numel():
-            stats.zero_()
-        return y, mean, rstd
+    mean, rstd = x.new_empty((N, groups), dtype=torch.float32), x.new_empty((N, groups), dtype=torch.float32)
+    if N == 0 or P == 0 or C == 0:
+        return y, mean.zero_(), rstd.zero_()
     nbytes = _gn_ws(N, P, C, groups, code, _GN_FWD)
-    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=x.device) if nbytes else None
-    with _on_device(x) as stream:
-        _lib.check(_lib.load().pgv_group_norm_act_fwd(x.data_ptr(), code, N, P, C, groups, _p(weight), _p(bias), eps, act, slope,
-                                                      y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _p(ws), nbytes, stream),
-                   "pgv_group_norm_act_fwd")
+    ws = x.new_empty(nbytes // 8, dtype=torch.float64) if nbytes else None
+    _lib.check(_lib.load().pgv_group_norm_act_fwd(x.data_ptr(), code, N, P, C, groups, _p(weight), _p(bias), eps, act, slope,
+                                                  y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _p(ws), nbytes, _raw_stream(x.get_device())),
+               "pgv_group_norm_act_fwd")
     return y, mean, rstd
 
 
@@ -1182,17 +1176,18 @@ def group_norm_act_fp8(x, groups, weight=None, bias=None, eps=1e-5, act=PGV_ACT_
     """``group_norm_act_fwd`` with the result written as the quantised operand of the next product: ``Fp8Blocks`` of the
     [items * pixels, channels] matrix, 'row' blocks, quantised from the float32 values (``pgv_group_norm_act_f8``)."""
     code, N, P, C = _gn_args("group_norm_act_fp8", x, groups, weight, bias, act)
+    if x.get_device() != _current_device():
+        return _elsewhere(x, group_norm_act_fp8, x, groups, weight, bias, eps, act, slope, fmt)
     if fmt not in F8_FORMATS:
         raise ValueError(f"group_norm_act_fp8: fmt is 'e4m3' or 'e5m2', got {fmt!r}")
-    t = _f8_alloc(N * P, C, 'row', fmt, x.device)
+    t = _f8_alloc(x, N * P, C, 'row', fmt)
     if x.numel() == 0:
         return t
     nbytes = _gn_ws(N, P, C, groups, code, _GN_F8)
-    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=x.device) if nbytes else None
-    with _on_device(x) as stream:
-        _lib.check(_lib.load().pgv_group_norm_act_f8(x.data_ptr(), code, N, P, C, groups, _p(weight), _p(bias), eps, act, slope,
-                                                     F8_FORMATS[fmt][0], t.q.data_ptr(), t.scale.data_ptr(), _p(ws), nbytes,
-                                                     stream), "pgv_group_norm_act_f8")
+    ws = x.new_empty(nbytes // 8, dtype=torch.float64) if nbytes else None
+    _lib.check(_lib.load().pgv_group_norm_act_f8(x.data_ptr(), code, N, P, C, groups, _p(weight), _p(bias), eps, act, slope,
+                                                 F8_FORMATS[fmt][0], t.q.data_ptr(), t.scale.data_ptr(), _p(ws), nbytes,
+                                                 _raw_stream(x.get_device())), "pgv_group_norm_act_f8")
     return t
 
 
@@ -1203,6 +1198,8 @@ def group_norm_act_bwd(gy, x, mean, rstd, groups, weight=None, bias=None, act=PG
     (``pgv_group_norm_act_bwd``)."""
     who = "group_norm_act_bwd"
     code, N, P, C = _gn_args(who, x, groups, weight, bias, act, gy, mean, rstd, ggamma, gbeta)
+    if x.get_device() != _current_device():
+        return _elsewhere(x, group_norm_act_bwd, gy, x, mean, rstd, groups, weight, bias, act, slope, need_params, ggamma, gbeta)
     if gy.shape != x.shape or gy.dtype != x.dtype or not gy.is_contiguous():
         raise ValueError(f"{who}: gy must be like x ({x.dtype}, {tuple(x.shape)}, contiguous)")
     _f32_vector(who, "mean", mean, N * groups)
@@ -1211,16 +1208,15 @@ def group_norm_act_bwd(gy, x, mean, rstd, groups, weight=None, bias=None, act=PG
     _f32_vector(who, "gbeta", gbeta, C)
     gx = torch.empty_like(x)
     if need_params:
-        ggamma = torch.empty(C, dtype=torch.float32, device=x.device) if ggamma is None else ggamma
-        gbeta = torch.empty(C, dtype=torch.float32, device=x.device) if gbeta is None else gbeta
+        ggamma = x.new_empty(C, dtype=torch.float32) if ggamma is None else ggamma
+        gbeta = x.new_empty(C, dtype=torch.float32) if gbeta is None else gbeta
     else:
         ggamma = gbeta = None
     if x.numel() == 0:
         return gx, ggamma.zero_() if need_params else None, gbeta.zero_() if need_params else None
     nbytes = _gn_ws(N, P, C, groups, code, _GN_BWD)
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device)
-    with _on_device(x) as stream:
-        _lib.check(_lib.load().pgv_group_norm_act_bwd(gy.data_ptr(), x.data_ptr(), code, N, P, C, groups, _p(weight), _p(bias),
-                                                      mean.data_ptr(), rstd.data_ptr(), act, slope, gx.data_ptr(), _p(ggamma),
-                                                      _p(gbeta), _p(ws), nbytes, stream), "pgv_group_norm_act_bwd")
+    ws = x.new_empty(nbytes // 4, dtype=torch.float32)
+    _lib.check(_lib.load().pgv_group_norm_act_bwd(gy.data_ptr(), x.data_ptr(), code, N, P, C, groups, _p(weight), _p(bias),
+                                                  mean.data_ptr(), rstd.data_ptr(), act, slope, gx.data_ptr(), _p(ggamma),
+                                                  _p(gbeta), _p(ws), nbytes, _raw_stream(x.get_device())), "pgv_group_norm_act_bwd")
     return gx, ggamma, gbeta
