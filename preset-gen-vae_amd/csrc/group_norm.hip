@@ -30,7 +30,19 @@ struct gn_args {
   float* part;          // partial sums (see each kernel)
   float* coef;          // backward: [N][G][2] = mean(h), mean(h xh)
   int W, tpr, slices;   // channels per workgroup, threads per row, pixel slices
+  uint32_t m_tpr, m_cg, m_per;   // fused kernels: magic numbers of tpr, cg and the pieces (or channels) of a group in a row
+  int lg;                        // log2 of the lanes that add up one group
 };
+
+// x / d for x d < 2^32 / d: the workgroup's own indices
+__device__ __forceinline__ int div_small(int x, int d, uint32_t magic) { return d == 1 ? x : (int)__umulhi((uint32_t)x, magic); }
+static inline uint32_t magic_of(int64_t d) { return d <= 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d); }
+
+// 1 / sqrt(v) within an ulp: the hardware's estimate and one Newton step
+__device__ __forceinline__ float rsqrt_(float v) {
+  const float y = __builtin_amdgcn_rsqf(v);
+  return fmaf(y * 0.5f, fmaf(-v * y, y, 1.f), y);
+}
 
 __device__ __forceinline__ float sigmoid_(float u) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
@@ -142,37 +154,53 @@ struct place {
   int c, n, r, rpp;
   int g[A];   // groups of the channels within the item
 };
-template <bool SAME>
+// LOCAL: c0 is a whole number of groups, and g counts from the workgroup's first one
+template <bool SAME, bool LOCAL = false>
 __device__ __forceinline__ place<SAME> my_place(const gn_args& p, int c0, int nt) {
   place<SAME> q;
-  const int row = threadIdx.x / p.tpr, j = threadIdx.x - row * p.tpr;
-  q.rpp = nt / p.tpr;
+  const int row = div_small(threadIdx.x, p.tpr, p.m_tpr), j = threadIdx.x - row * p.tpr;
+  q.rpp = div_small(nt, p.tpr, p.m_tpr);
   q.r = row;
   q.c = c0 + 8 * j;
   const int end = min(c0 + p.W, p.C);
   q.n = q.r < q.rpp ? max(0, min(8, end - q.c)) : 0;
 #pragma unroll
-  for (int i = 0; i < q.A; ++i) q.g[i] = i < q.n ? (q.c + i) / p.cg : 0;
+  for (int i = 0; i < q.A; ++i) q.g[i] = i >= q.n ? 0 : LOCAL ? div_small(8 * j + i, p.cg, p.m_cg) : (q.c + i) / p.cg;
   return q;
 }
-// the per-channel vectors of a place; channels beyond the valid ones normalise to 0
+// the per-channel vectors of a place; channels beyond the valid ones normalise to 0.  ar = gamma rstd: u = (x - mean) ar + beta
+// is two operations, and subtracting the mean first loses nothing when it is far from zero.
 template <bool SAME>
 struct chan {
-  float ga[8], be[8], mu[SAME ? 1 : 8], rs[SAME ? 1 : 8];
+  float ga[8], be[8], mu[SAME ? 1 : 8], rs[SAME ? 1 : 8], ar[8];
 };
-template <bool SAME>
-__device__ __forceinline__ void load_affine(const gn_args& p, const place<SAME>& q, chan<SAME>& k) {
+template <bool VEC>
+__device__ __forceinline__ void load8f(const float* __restrict__ v, int c, int n, float fill, float (&o)[8]) {
+  if (v == nullptr) {   // (uniform)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    k.ga[i] = i < q.n && p.gamma ? p.gamma[q.c + i] : (i < q.n ? 1.f : 0.f);
-    k.be[i] = i < q.n && p.beta ? p.beta[q.c + i] : 0.f;
+    for (int i = 0; i < 8; ++i) o[i] = i < n ? fill : 0.f;
+  } else if constexpr (VEC) {
+    f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+    if (n > 0) a = reinterpret_cast<const f32x4*>(v + c)[0], b = reinterpret_cast<const f32x4*>(v + c)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = a[i], o[4 + i] = b[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = i < n ? v[c + i] : 0.f;
   }
 }
+template <bool VEC, bool SAME>
+__device__ __forceinline__ void load_affine(const gn_args& p, const place<SAME>& q, chan<SAME>& k) {
+  load8f<VEC>(p.gamma, q.c, q.n, 1.f, k.ga);
+  load8f<VEC>(p.beta, q.c, q.n, 0.f, k.be);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) k.ar[i] = k.ga[i] * k.rs[SAME ? 0 : i];
+}
 template <bool SAME>
-__device__ __forceinline__ void load_stats(const gn_args& p, const place<SAME>& q, int item, chan<SAME>& k) {
+__device__ __forceinline__ void load_stats(const gn_args& p, const place<SAME>& q, int item, int gfirst, chan<SAME>& k) {
 #pragma unroll
   for (int i = 0; i < q.A; ++i) {
-    const int64_t g = (int64_t)item * p.G + q.g[i];
+    const int64_t g = (int64_t)item * p.G + gfirst + q.g[i];
     k.mu[i] = i < q.n ? p.mean[g] : 0.f;
     k.rs[i] = i < q.n ? p.rstd[g] : 0.f;
   }
@@ -183,7 +211,7 @@ template <bool VEC, bool Q, int FMT, bool SAME, typename T>
 __device__ __forceinline__ void put(const gn_args& p, const place<SAME>& q, const chan<SAME>& k, int64_t pix, const raw8<T>& x) {
   float u[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) u[i] = fmaf((x[i] - k.mu[SAME ? 0 : i]) * k.rs[SAME ? 0 : i], k.ga[i], k.be[i]);
+  for (int i = 0; i < 8; ++i) u[i] = fmaf(x[i] - k.mu[SAME ? 0 : i], k.ar[i], k.be[i]);
   act8(u, p.act, p.slope);
   if constexpr (!Q) {
     store8<VEC>((T*)p.y + pix * p.C + q.c, q.n, u);
@@ -204,18 +232,22 @@ __device__ __forceinline__ void put(const gn_args& p, const place<SAME>& q, cons
 
 // Sums over the entries of every group: L neighbouring lanes per group (a power of two, at most 64), each over every L-th entry.
 // at(g, e): entry e < cnt(g) of local group g; done(g, sum): called by one lane.
-template <typename V, typename At, typename Cnt, typename Done>
-__device__ __forceinline__ void sum_groups(int groups, int nt, At at, Cnt cnt, Done done) {
-  int lg = 31 - __builtin_clz(max(1, nt / groups));
-  lg = lg > 6 ? 6 : lg;
-  const int L = 1 << lg, s = threadIdx.x & (L - 1);
-  for (int g = threadIdx.x >> lg; g < ((groups + (nt >> lg) - 1) / (nt >> lg)) * (nt >> lg); g += nt >> lg) {
+template <int NT, typename V, typename At, typename Cnt, typename Done>
+__device__ __forceinline__ void sum_groups(int groups, int lg, At at, Cnt cnt, Done done) {
+  const int L = 1 << lg, s = threadIdx.x & (L - 1), step = NT >> lg;
+  for (int g0 = 0; g0 < groups; g0 += step) {
+    const int g = g0 + (threadIdx.x >> lg);
     V v{};
     const int n = g < groups ? cnt(g) : 0;
     for (int e = s; e < n; e += L) v.add(at(g, e));
     for (int o = L >> 1; o > 0; o >>= 1) v.add(v.from(o));
     if (s == 0 && g < groups) done(g, v);
   }
+}
+static inline int lanes_log2(int64_t nt, int64_t groups) {
+  int lg = 0;
+  while (lg < 6 && (nt >> (lg + 1)) >= groups) ++lg;
+  return lg;
 }
 struct sum1 {
   float a;
@@ -241,24 +273,47 @@ struct sum2 {
 constexpr int MAXG = 256;   // groups of a workgroup of the fused kernels
 
 // ---- forward, fused: grid (column blocks of W channels, items) -----------------------------------------------------------
-template <typename T, int NT, int KV, bool VEC, bool Q, int FMT, bool SAME>
+// A thread holds KV pieces in registers and KL more in LDS (16 bytes each: 16-bit types only).
+template <typename T, int NT, int KV, int KL, bool VEC, bool Q, int FMT, bool SAME>
 __global__ __launch_bounds__(NT) void gn_fwd_fused_kernel(gn_args p) {
   constexpr int A = SAME ? 1 : 8;
+  extern __shared__ __attribute__((aligned(16))) i32x4 held[];   // [KL][NT]
   __shared__ __attribute__((aligned(16))) float val[NT * A];
   __shared__ float gs[2][MAXG];
   const int tid = threadIdx.x, item = blockIdx.y, c0 = blockIdx.x * p.W;
-  const place<SAME> q = my_place<SAME>(p, c0, NT);
-  const int groups = min(p.W, p.C - c0) / p.cg, gfirst = c0 / p.cg;
-  const T* x = (const T*)p.x + (int64_t)item * p.P * p.C;
+  const place<SAME> q = my_place<SAME, true>(p, c0, NT);
+  const int gfirst = blockIdx.x * (p.W / p.cg), groups = min(p.W / p.cg, p.G - gfirst);
+  const T* x = (const T*)p.x + (int64_t)item * p.P * p.C;   // (the item's bytes are addressed with 32 bits: make_gn_plan)
+  const uint32_t at0 = (uint32_t)(q.r * p.C + q.c), step = (uint32_t)(q.rpp * p.C);
+  auto get = [&](int k) {
+    raw8<T> d;
+    if (q.r + k * q.rpp < p.P && q.n > 0)
+      d = load_raw<VEC>(x + (at0 + k * step), q.n);
+    else
+      d.clear();
+    return d;
+  };
+  if constexpr (KL > 0) {
+#pragma unroll
+    for (int h = 0; h < KL; h += 4) {
+      raw8<T> e[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) e[k] = get(KV + h + k);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        held[(h + k) * NT + tid] = i32x4{(int)e[k].w[0], (int)e[k].w[1], (int)e[k].w[2], (int)e[k].w[3]};
+    }
+  }
   raw8<T> d[KV];
 #pragma unroll
-  for (int k = 0; k < KV; ++k) {
-    const int r = q.r + k * q.rpp;
-    if (r < p.P && q.n > 0)
-      d[k] = load_raw<VEC>(x + (int64_t)r * p.C + q.c, q.n);
-    else
-      d[k].clear();
-  }
+  for (int k = 0; k < KV; ++k) d[k] = get(k);
+  auto from_lds = [&](int k) {   // (a thread reads what it wrote: no barrier)
+    const i32x4 v = held[k * NT + tid];
+    raw8<T> e;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e.w[i] = (uint32_t)v[i];
+    return e;
+  };
   chan<SAME> ch;
   const float inv_n = 1.f / ((float)p.P * (float)p.cg);
   const int per = SAME ? p.cg >> 3 : p.cg, pitch = SAME ? p.tpr : p.tpr * 8;
@@ -272,50 +327,58 @@ __global__ __launch_bounds__(NT) void gn_fwd_fused_kernel(gn_args p) {
     float s[A];
 #pragma unroll
     for (int i = 0; i < A; ++i) s[i] = 0.f;
+    auto take = [&](const raw8<T>& e) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = e[i] - ch.mu[SAME ? 0 : i];
+        if (pass)
+          s[SAME ? 0 : i] = fmaf(v, v, s[SAME ? 0 : i]);
+        else
+          s[SAME ? 0 : i] += v;
+      }
+    };
 #pragma unroll
     for (int k = 0; k < KV; ++k)
-      if (q.r + k * q.rpp < p.P)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float v = d[k][i] - ch.mu[SAME ? 0 : i];
-          s[SAME ? 0 : i] += pass ? v * v : v;
-        }
+      if (q.r + k * q.rpp < p.P) take(d[k]);
+    if constexpr (KL > 0)
+#pragma unroll 2
+      for (int k = 0; k < KL; ++k)
+        if (q.r + (KV + k) * q.rpp < p.P) take(from_lds(k));
     if (pass) __syncthreads();   // the readers of val of pass 0 are done
 #pragma unroll
     for (int i = 0; i < A; ++i) val[tid * A + i] = i < q.n ? s[i] : 0.f;
     __syncthreads();
-    sum_groups<sum1>(groups, NT,
+    sum_groups<NT, sum1>(groups, p.lg,
         [&](int g, int e) {
-          const int r = e / per;
+          const int r = div_small(e, per, p.m_per);
           sum1 v;
           v.a = val[r * pitch + g * per + (e - r * per)];
           return v;
         },
-        [&](int) { return q.rpp * per; }, [&](int g, const sum1& v) { gs[pass][g] = v.a; });
+        [&](int) { return q.rpp * per; },
+        [&](int g, const sum1& v) {
+          const float m = pass ? rsqrt_(v.a * inv_n + p.eps) : v.a * inv_n;
+          gs[pass][g] = m;
+          if (p.mean) (pass ? p.rstd : p.mean)[(int64_t)item * p.G + gfirst + g] = m;
+        });
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < A; ++i) {
-      const int g = i < q.n ? q.g[i] - gfirst : 0;
-      if (pass == 0)
-        ch.mu[i] = i < q.n ? gs[0][g] * inv_n : 0.f;
-      else
-        ch.rs[i] = i < q.n ? 1.f / sqrtf(gs[1][g] * inv_n + p.eps) : 0.f;
-    }
+    for (int i = 0; i < A; ++i) (pass ? ch.rs : ch.mu)[i] = i < q.n ? gs[pass][q.g[i]] : 0.f;
   }
-  if (p.mean)
-    for (int g = tid; g < groups; g += NT) {
-      const int64_t o = (int64_t)item * p.G + gfirst + g;
-      p.mean[o] = gs[0][g] * inv_n;
-      p.rstd[o] = 1.f / sqrtf(gs[1][g] * inv_n + p.eps);
-    }
   if (q.r >= q.rpp) return;
-  load_affine(p, q, ch);
+  load_affine<VEC>(p, q, ch);
 #pragma unroll
   for (int k = 0; k < KV; ++k) {
     const int r = q.r + k * q.rpp;
     d[k].forget();
     if (r < p.P && (Q || q.n > 0)) put<VEC, Q, FMT>(p, q, ch, (int64_t)item * p.P + r, d[k]);
   }
+  if constexpr (KL > 0)
+#pragma unroll 1
+    for (int k = 0; k < KL; ++k) {
+      const int r = q.r + (KV + k) * q.rpp;
+      if (r < p.P && (Q || q.n > 0)) put<VEC, Q, FMT>(p, q, ch, (int64_t)item * p.P + r, from_lds(k));
+    }
 }
 
 // ---- forward, two-pass --------------------------------------------------------------------------------------------------
@@ -353,7 +416,7 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(gn_args p) {
   __syncthreads();
   sum2<double>* out = (sum2<double>*)p.part + ((int64_t)item * (p.slices * gridDim.y) + (int64_t)blockIdx.y * p.slices + slice) * p.G;
   const int cend = min(c0 + p.W, p.C), pitch = SAME ? p.tpr : p.tpr * 8;
-  sum_groups<sum2<double>>(p.G, 256,
+  sum_groups<256, sum2<double>>(p.G, p.lg,
       [&](int g, int e) {
         const int lo = max(g * p.cg, c0), w = (min((g + 1) * p.cg, cend) - lo) / (SAME ? 8 : 1), r = e / w;
         return val[r * pitch + (lo - c0) / (SAME ? 8 : 1) + (e - r * w)];
@@ -387,8 +450,8 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(gn_args p) {
   const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
   const T* x = (const T*)p.x + (int64_t)item * p.P * p.C + q.c;
   chan<SAME> ch;
-  load_affine(p, q, ch);
-  load_stats(p, q, item, ch);
+  load_stats(p, q, item, 0, ch);
+  load_affine<VEC>(p, q, ch);
   auto get = [&](int r) {
     raw8<T> d;
     if (!Q || q.n > 0)
@@ -416,8 +479,9 @@ __device__ __forceinline__ void grads8(const gn_args& p, const chan<SAME>& k, co
   float u[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    xh[i] = (x[i] - k.mu[SAME ? 0 : i]) * k.rs[SAME ? 0 : i];
-    u[i] = fmaf(xh[i], k.ga[i], k.be[i]);
+    const float v = x[i] - k.mu[SAME ? 0 : i];
+    xh[i] = v * k.rs[SAME ? 0 : i];
+    u[i] = fmaf(v, k.ar[i], k.be[i]);
     du[i] = gy[i];
   }
   act_grad8(du, u, p.act, p.slope);
@@ -490,24 +554,25 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(gn_args p) {
   float* tot = sm + NT * 16;       // [2][width]
   __shared__ float gs[2][MAXG];
   const int item = blockIdx.y, c0 = blockIdx.x * p.W, width = min(p.W, p.C - c0);
-  const place<SAME> q = my_place<SAME>(p, c0, NT);
+  const place<SAME> q = my_place<SAME, true>(p, c0, NT);
+  const int gfirst = blockIdx.x * (p.W / p.cg);
   const T* x = (const T*)p.x + (int64_t)item * p.P * p.C;
   const T* gy = (const T*)p.gy + (int64_t)item * p.P * p.C;
+  const uint32_t at0 = (uint32_t)(q.r * p.C + q.c), step = (uint32_t)(q.rpp * p.C);
   raw8<T> d[KV], e[KV];
 #pragma unroll
   for (int k = 0; k < KV; ++k) {
-    const int r = q.r + k * q.rpp;
-    if (r < p.P && q.n > 0) {
-      d[k] = load_raw<VEC>(x + (int64_t)r * p.C + q.c, q.n);
-      e[k] = load_raw<VEC>(gy + (int64_t)r * p.C + q.c, q.n);
+    if (q.r + k * q.rpp < p.P && q.n > 0) {
+      d[k] = load_raw<VEC>(x + (at0 + k * step), q.n);
+      e[k] = load_raw<VEC>(gy + (at0 + k * step), q.n);
     } else {
       d[k].clear();
       e[k].clear();
     }
   }
   chan<SAME> ch;
-  load_affine(p, q, ch);
-  load_stats(p, q, item, ch);
+  load_stats(p, q, item, gfirst, ch);
+  load_affine<VEC>(p, q, ch);
   float a[8], b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) a[i] = 0.f, b[i] = 0.f;
@@ -523,7 +588,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(gn_args p) {
   for (int k = 0; k < KV; ++k) d[k].forget(), e[k].forget();
   channel_sums<NT>(p, q.n, q.rpp, a, b, val, tot, width);
   const float inv_n = 1.f / ((float)p.P * (float)p.cg);
-  sum_groups<sum2<float>>(width / p.cg, NT,
+  sum_groups<NT, sum2<float>>(min(p.W / p.cg, p.G - gfirst), p.lg,
       [&](int g, int i) {
         const int c = g * p.cg + i;
         const float ga = p.gamma ? p.gamma[c0 + c] : 1.f;
@@ -543,9 +608,8 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(gn_args p) {
   float c1[q.A], c2[q.A];
 #pragma unroll
   for (int i = 0; i < q.A; ++i) {
-    const int g = i < q.n ? q.g[i] - c0 / p.cg : 0;
-    c1[i] = gs[0][g];
-    c2[i] = gs[1][g];
+    c1[i] = gs[0][q.g[i]];
+    c2[i] = gs[1][q.g[i]];
   }
 #pragma unroll
   for (int k = 0; k < KV; ++k) {
@@ -566,8 +630,8 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(gn_args p) {
   const T* x = (const T*)p.x + base;
   const T* gy = (const T*)p.gy + base;
   chan<SAME> ch;
-  load_affine(p, q, ch);
-  load_stats(p, q, item, ch);
+  load_stats(p, q, item, 0, ch);
+  load_affine<VEC>(p, q, ch);
   float a[8], b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) a[i] = 0.f, b[i] = 0.f;
@@ -649,8 +713,8 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(gn_args p) {
   const T* x = (const T*)p.x + base;
   const T* gy = (const T*)p.gy + base;
   chan<SAME> ch;
-  load_affine(p, q, ch);
-  load_stats(p, q, item, ch);
+  load_stats(p, q, item, 0, ch);
+  load_affine<VEC>(p, q, ch);
   float c1[q.A], c2[q.A];
 #pragma unroll
   for (int i = 0; i < q.A; ++i) {
@@ -665,24 +729,25 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(gn_args p) {
   }
 }
 
-// gbeta / ggamma: rows [rows][2][C] of channel sums, added in a fixed order (8 interleaved chains, then their sum)
-__global__ __launch_bounds__(256) void gn_param_grads_kernel(const float* __restrict__ part, int64_t rows, int C,
-                                                             float* __restrict__ ggamma, float* __restrict__ gbeta) {
-  __shared__ double red[8][64];
+// gbeta / ggamma: rows [rows][2][C] of channel sums, added in a fixed order (32 interleaved chains, then their sum)
+__global__ __launch_bounds__(1024) void gn_param_grads_kernel(const float* __restrict__ part, int rows, int C,
+                                                              float* __restrict__ ggamma, float* __restrict__ gbeta) {
+  __shared__ double red[32][65];
   const int l = threadIdx.x & 31, ph = threadIdx.x >> 5, c = blockIdx.x * 32 + l;
   double a = 0.0, b = 0.0;
   if (c < C)
-#pragma unroll 8
-    for (int64_t r = ph; r < rows; r += 8) {
-      a += (double)part[r * 2 * C + c];
-      b += (double)part[(r * 2 + 1) * C + c];
+#pragma unroll 4
+    for (int r = ph; r < rows; r += 32) {
+      a += (double)part[(int64_t)r * 2 * C + c];
+      b += (double)part[((int64_t)r * 2 + 1) * C + c];
     }
   red[ph][l] = a;
   red[ph][32 + l] = b;
   __syncthreads();
   if (threadIdx.x < 64) {
     double s = 0.0;
-    for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i) s += red[i][threadIdx.x];
     float* out = threadIdx.x < 32 ? gbeta : ggamma;
     if (out && c < C) out[c] = (float)s;
   }
@@ -691,8 +756,9 @@ __global__ __launch_bounds__(256) void gn_param_grads_kernel(const float* __rest
 // ---- which scheme: a function of the sizes and the element size -----------------------------------------------------------
 struct gn_plan {
   bool fused;
-  int W, tpr, nt, kv;      // fused
-  int slices, colblocks;   // two-pass
+  int W, tpr, colblocks, lg;
+  int nt, kv;      // fused: threads, pieces per thread
+  int slices;      // two-pass
 };
 
 int64_t gcd_(int64_t a, int64_t b) {
@@ -719,13 +785,17 @@ gn_plan make_gn_plan(int64_t N, int64_t P, int64_t C, int64_t G, int esize, int 
   if (kind == 1) tpr = pgv_cdiv(W, F8B) * 16;
   const int64_t groups = pgv_cdiv(W, cg);
   // {threads, pieces of 8 values a thread holds, bytes per value at most}: the pieces take 8 or 4 registers each, twice that for
-  // the backward pass, out of 128 with 1024 threads and 512 with 256
-  static const int fwd[][3] = {{256, 1, 4}, {256, 4, 4}, {256, 8, 4}, {1024, 4, 4}, {1024, 8, 4}, {1024, 16, 2}, {1024, 24, 2}};
-  static const int bwd[][3] = {{256, 1, 4}, {256, 4, 4}, {256, 8, 4}, {1024, 4, 4}, {1024, 8, 2}};
-  if (groups <= MAXG)
-    for (int i = 0; i < (kind == 2 ? 5 : 7); ++i) {
+  // the backward pass, out of 128 with 1024 threads, 256 with 512 and 512 with fewer; pieces 17 to 24 are held in LDS.  One wave
+  // per workgroup saves the barriers and most of what a thread does besides its values, where there are workgroups enough to
+  // fill the device without more (160 x 16 blocks of 12 pixels: 8 us against 26 us with 256 threads).
+  static const int fwd[][3] = {{64, 1, 4},  {64, 4, 4},   {64, 8, 4},   {256, 1, 4},   {256, 4, 4},
+                               {256, 8, 4}, {1024, 4, 4}, {1024, 8, 4}, {1024, 16, 2}, {1024, 24, 2}};
+  static const int bwd[][3] = {{64, 1, 4}, {64, 4, 4}, {64, 8, 4}, {256, 1, 4}, {256, 4, 4}, {256, 8, 4}, {512, 8, 4}, {512, 16, 2}};
+  const bool many = N * pgv_cdiv(C, W) >= 1024;
+  if (groups <= MAXG && P * C * esize < (1ll << 31))
+    for (int i = many ? 0 : 3; i < (kind == 2 ? 8 : 10); ++i) {
       const int* c = kind == 2 ? bwd[i] : fwd[i];
-      if (esize > c[2]) continue;
+      if (esize > c[2] || (c[1] == 24 && cg % 8)) continue;   // (groups of other widths need the LDS for their reductions)
       const int64_t rpp = c[0] / tpr;
       if (rpp >= 1 && P <= rpp * c[1]) {
         r.fused = true;
@@ -734,12 +804,14 @@ gn_plan make_gn_plan(int64_t N, int64_t P, int64_t C, int64_t G, int esize, int 
         r.nt = c[0];
         r.kv = c[1];
         r.colblocks = (int)pgv_cdiv(C, W);
+        r.lg = lanes_log2(r.nt, groups);
         return r;
       }
     }
   r.W = (int)(C < 2048 ? C : 2048);
   r.tpr = (int)(kind == 1 ? pgv_cdiv(r.W, F8B) * 16 : pgv_cdiv(r.W, 8));
   r.colblocks = (int)pgv_cdiv(C, r.W);
+  r.lg = lanes_log2(256, G);
   const int64_t rpp = 256 / r.tpr;
   int64_t s = pgv_cdiv(2048, N * r.colblocks);
   const int64_t most = pgv_cdiv(P, rpp * 4);
@@ -758,20 +830,42 @@ int gn_check(const char* who, int64_t N, int64_t P, int64_t C, int64_t G, int dt
   return PGV_OK;
 }
 
-template <typename T, bool VEC, bool Q, int FMT, bool SAME>
-int gn_forward(gn_args p, const gn_plan& pl, hipStream_t st) {
+void set_plan(gn_args& p, const gn_plan& pl, bool same) {
   p.W = pl.W;
   p.tpr = pl.tpr;
   p.slices = pl.slices;
+  p.lg = pl.lg;
+  p.m_tpr = magic_of(pl.tpr);
+  p.m_cg = magic_of(p.cg);
+  p.m_per = magic_of(same ? p.cg / 8 : p.cg);
+}
+
+template <typename T, bool VEC, bool Q, int FMT, bool SAME>
+int gn_forward(gn_args p, const gn_plan& pl, hipStream_t st) {
+  set_plan(p, pl, SAME);
   if (pl.fused) {
     const dim3 grid((unsigned)pl.colblocks, (unsigned)p.N);
-#define PGV_F(NT, KV) gn_fwd_fused_kernel<T, NT, KV, VEC, Q, FMT, SAME><<<grid, NT, 0, st>>>(p)
-    if (pl.nt == 256)
+#define PGV_F(NT, KV) gn_fwd_fused_kernel<T, NT, KV, 0, VEC, Q, FMT, SAME><<<grid, NT, 0, st>>>(p)
+    if (pl.nt == 64)
+      pl.kv == 1 ? PGV_F(64, 1) : pl.kv == 4 ? PGV_F(64, 4) : PGV_F(64, 8);
+    else if (pl.nt == 256)
       pl.kv == 1 ? PGV_F(256, 1) : pl.kv == 4 ? PGV_F(256, 4) : PGV_F(256, 8);
     else if (pl.kv <= 8)
       pl.kv == 4 ? PGV_F(1024, 4) : PGV_F(1024, 8);
-    else if constexpr (sizeof(T) == 2)
-      pl.kv == 16 ? PGV_F(1024, 16) : PGV_F(1024, 24);
+    else if constexpr (sizeof(T) == 2) {
+      if (pl.kv == 16) {
+        PGV_F(1024, 16);
+      } else if constexpr (SAME) {
+        auto k = gn_fwd_fused_kernel<T, 1024, 16, 8, VEC, Q, FMT, SAME>;
+        constexpr int lds = 8 * 1024 * 16;
+        static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (once != hipSuccess) {
+          pgv_set_error("pgv_group_norm_act: %d bytes of LDS refused: %s", lds, hipGetErrorString(once));
+          return PGV_E_LAUNCH;
+        }
+        k<<<grid, 1024, lds, st>>>(p);
+      }
+    }
 #undef PGV_F
     return PGV_OK;
   }
@@ -797,21 +891,23 @@ int launch_bwd_fused(const gn_args& p, dim3 grid, hipStream_t st) {
 
 template <typename T, bool VEC, bool SAME>
 int gn_backward(gn_args p, const gn_plan& pl, float* ggamma, float* gbeta, hipStream_t st) {
-  p.W = pl.W;
-  p.tpr = pl.tpr;
-  p.slices = pl.slices;
+  set_plan(p, pl, SAME);
   const float* item_tot = p.part;
   if (pl.fused) {
     const dim3 grid((unsigned)pl.colblocks, (unsigned)p.N);
     int rc = PGV_OK;
-    if (pl.nt == 256)
+    if (pl.nt == 64)
+      rc = pl.kv == 1   ? launch_bwd_fused<T, 64, 1, VEC, SAME>(p, grid, st)
+           : pl.kv == 4 ? launch_bwd_fused<T, 64, 4, VEC, SAME>(p, grid, st)
+                        : launch_bwd_fused<T, 64, 8, VEC, SAME>(p, grid, st);
+    else if (pl.nt == 256)
       rc = pl.kv == 1   ? launch_bwd_fused<T, 256, 1, VEC, SAME>(p, grid, st)
            : pl.kv == 4 ? launch_bwd_fused<T, 256, 4, VEC, SAME>(p, grid, st)
                         : launch_bwd_fused<T, 256, 8, VEC, SAME>(p, grid, st);
-    else if (pl.kv == 4)
-      rc = launch_bwd_fused<T, 1024, 4, VEC, SAME>(p, grid, st);
+    else if (pl.kv == 8)
+      rc = launch_bwd_fused<T, 512, 8, VEC, SAME>(p, grid, st);
     else if constexpr (sizeof(T) == 2)
-      rc = launch_bwd_fused<T, 1024, 8, VEC, SAME>(p, grid, st);
+      rc = launch_bwd_fused<T, 512, 16, VEC, SAME>(p, grid, st);
     if (rc != PGV_OK) return rc;
   } else {
     const dim3 grid((unsigned)pl.slices, (unsigned)pl.colblocks, (unsigned)p.N);
@@ -824,7 +920,7 @@ int gn_backward(gn_args p, const gn_plan& pl, float* ggamma, float* gbeta, hipSt
     item_tot = tot;
   }
   if (ggamma || gbeta)
-    gn_param_grads_kernel<<<dim3((unsigned)pgv_cdiv(p.C, 32)), 256, 0, st>>>(item_tot, p.N, p.C, ggamma, gbeta);
+    gn_param_grads_kernel<<<dim3((unsigned)pgv_cdiv(p.C, 32)), 1024, 0, st>>>(item_tot, p.N, p.C, ggamma, gbeta);
   return PGV_OK;
 }
 
@@ -863,14 +959,12 @@ static int gn_fwd_any(const char* who, const void* x, int dtype, int64_t N, int6
     float* tail = (float*)((char*)workspace + need - 8 * N * G);
     p.mean = tail, p.rstd = tail + N * G;
   }
-  const bool vec = C % 8 == 0 && (uintptr_t)x % 16 == 0 && (q || (uintptr_t)y % 16 == 0);
+  const bool vec = C % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)gamma % 16 == 0 && (uintptr_t)beta % 16 == 0 && (q || (uintptr_t)y % 16 == 0);
   hipStream_t st = pgv_stream(stream);
   int r;
-  // (C/G a multiple of 8 makes C one: rows that are not 16-byte pieces then come from an unaligned base alone)
   const bool same = p.cg % 8 == 0;
-#define PGV_T(T, Q, FMT)                                                                                    \
-  (vec ? (same ? gn_forward<T, true, Q, FMT, true>(p, pl, st) : gn_forward<T, true, Q, FMT, false>(p, pl, st)) \
-       : gn_forward<T, false, Q, FMT, false>(p, pl, st))
+#define PGV_V(T, VEC, Q, FMT) (same ? gn_forward<T, VEC, Q, FMT, true>(p, pl, st) : gn_forward<T, VEC, Q, FMT, false>(p, pl, st))
+#define PGV_T(T, Q, FMT) (vec ? PGV_V(T, true, Q, FMT) : PGV_V(T, false, Q, FMT))
 #define PGV_D(Q, FMT) (dtype == PGV_DT_F32 ? PGV_T(float, Q, FMT) : dtype == PGV_DT_BF16 ? PGV_T(__bf16, Q, FMT) : PGV_T(_Float16, Q, FMT))
   if (!q)
     r = PGV_D(false, PGV_F8_E4M3);
@@ -878,6 +972,7 @@ static int gn_fwd_any(const char* who, const void* x, int dtype, int64_t N, int6
     r = fmt == PGV_F8_E4M3 ? PGV_D(true, PGV_F8_E4M3) : PGV_D(true, PGV_F8_E5M2);
 #undef PGV_D
 #undef PGV_T
+#undef PGV_V
   if (r != PGV_OK) return r;
   PGV_CHECK_LAUNCH(who);
   return PGV_OK;
@@ -919,7 +1014,7 @@ extern "C" int pgv_group_norm_act_bwd(const void* gy, const void* x, int dtype, 
   p.x = x, p.gy = gy, p.gx = gx, p.gamma = gamma, p.beta = beta, p.slope = slope, p.act = act;
   p.mean = const_cast<float*>(mean), p.rstd = const_cast<float*>(rstd);
   p.part = (float*)workspace;
-  const bool vec = C % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)gy % 16 == 0 && (uintptr_t)gx % 16 == 0;
+  const bool vec = C % 8 == 0 && (uintptr_t)gamma % 16 == 0 && (uintptr_t)beta % 16 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)gy % 16 == 0 && (uintptr_t)gx % 16 == 0;
   hipStream_t st = pgv_stream(stream);
   const bool same = p.cg % 8 == 0;
 #define PGV_T(T)                                                                                                  \
