@@ -7,10 +7,9 @@
 // The order of k inside a block is free as long as both operands use the same: every lane reads 32 consecutive bytes.
 //
 // Three kernels:
-//   skinny  few rows (m): bound by reading b once.  No LDS on the way in: b goes from memory straight into the fragment
-//           registers, the reduction is spread over the 8 waves of a workgroup and over workgroups, the partial sums meet in
-//           LDS.  The fused form also quantises the rows of a in registers: a lane's 32 values of a block are in its
-//           fragment, the block's maximum is two shuffles away.
+//   skinny  few rows (m): bound by reading b once.  b goes from memory straight into the fragment registers, the reduction is
+//           spread over the 8 waves of a workgroup and over workgroups, the partial sums meet in LDS.  The fused form also
+//           quantises the rows of a.
 //   tile    everything else: BM x BN x 128-byte stages in LDS, filled by LDS-DMA, double buffered.
 //   join    adds the fp32 partial results of a reduction that was split over workgroups, in the order of the splits.
 #include "f8_common.h"
@@ -86,145 +85,116 @@ struct skinny_args {
   float* part;            // [splits][M][N] when splits > 1
 };
 
-// 32 consecutive values of a row, as they lie in memory (VEC: 16-byte aligned), then as 32 bytes + their block's scale
-template <typename T>
-struct raw32 {
-  T v[32];
-};
-template <typename T, bool VEC>
-__device__ __forceinline__ raw32<T> load32(const T* __restrict__ p, int n) {
-  raw32<T> r;
-  constexpr int E = 16 / sizeof(T);
-  typedef T te __attribute__((ext_vector_type(E)));
-  if (VEC && n >= 32) {
-#pragma unroll
-    for (int i = 0; i < 32 / E; ++i) {
-      const te t = reinterpret_cast<const te*>(p)[i];
-#pragma unroll
-      for (int j = 0; j < E; ++j) r.v[i * E + j] = t[j];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) r.v[i] = i < n ? p[i] : (T)0.f;
-  }
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ i32x8 quant_frag(const raw32<T>& r, float& scale) {
-  i32x8 f;
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) m = max(m, f8_abs_bits((float)r.v[i]));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-  float inv;
-  f8_scale<PGV_F8_E4M3>(m, scale, inv);
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    f[i] = f8_pack4<PGV_F8_E4M3>((float)r.v[4 * i] * inv, (float)r.v[4 * i + 1] * inv, (float)r.v[4 * i + 2] * inv,
-                                 (float)r.v[4 * i + 3] * inv);
-  return f;
+// lanes of a wave have exchanged data through LDS: what they wrote before is seen after (the LDS serves a wave in order; this
+// keeps the compiler's order too)
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// T = uint8_t: a is 8-bit rows of format FA; else its values are quantised here (e4m3).  MF x NF tiles of 16 x 16 per wave;
-// U blocks of the reduction are requested before the first is used: a wave has few of them, so their latencies must overlap.
-template <typename T, int FA, bool F32, bool VEC, int MF, int NF, int U>
+// T = uint8_t: a is 8-bit rows of format FA; else its values are quantised here (e4m3), by every wave for its own blocks: 16
+// lanes x 8 values make a block, four blocks of a row at a time, and the bytes change lanes through LDS (a lane of the matrix
+// instruction takes 32 neighbours).  No barrier: a wave reads what it wrote.  For one row that is 16 times less work than
+// quantising in the fragment layout, where 15 of 16 rows are none.
+// MF tiles of 16 x 16 per wave; U blocks of the reduction are requested before the first is used: a wave has few of them, so
+// their latencies must overlap.
+template <typename T, int FA, bool F32, bool VEC, int MF, int U>
 __global__ __launch_bounds__(64 * SW) void skinny_kernel(skinny_args p) {
   constexpr bool Q = sizeof(T) == 1;
-  constexpr int GRP = NF * MF < 4 ? NF * MF : 4;   // tiles that meet in LDS at a time
-  __shared__ __attribute__((aligned(16))) float lds[SW * GRP * 256];
+  static_assert(Q || (MF == 1 && U == 4), "the fused form holds 16 rows and four blocks");
+  constexpr int ROW = 128 + 16;                     // bytes of a row of the exchange image: 16-byte pieces of 8 rows in 8 banks
+  constexpr int XCH = Q ? 0 : U * (16 * ROW + 64);  // a wave's image: U blocks of 16 rows, U x 16 scales
+  constexpr int SUM = MF * 256 * (int)sizeof(float);
+  __shared__ __attribute__((aligned(16))) uint8_t lds[SW * (XCH > SUM ? XCH : SUM)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * (16 * NF), m0 = blockIdx.y * (16 * MF), split = blockIdx.z;
+  const int n0 = blockIdx.x * 16, split = blockIdx.z;
   const int kb0 = (int)((int64_t)p.Kb * split / p.splits), kb1 = (int)((int64_t)p.Kb * (split + 1) / p.splits);
   const int64_t Kp = (int64_t)p.Kb * F8B;
-  const uint8_t* bp[NF];
-  const float* sbp[NF];
+  const uint8_t* bp = p.b + min(n0 + l16, p.N - 1) * Kp + g * 32;
+  const float* sbp = p.sb + (int64_t)(n0 / F8B) * p.Kb;
+  uint8_t* img = lds + wave * XCH;
+  float* img_s = reinterpret_cast<float*>(img + U * 16 * ROW);
+  f32x4 acc[MF];
 #pragma unroll
-  for (int f = 0; f < NF; ++f) {
-    const int n = min(n0 + 16 * f + l16, p.N - 1);
-    bp[f] = p.b + n * Kp + g * 32;
-    sbp[f] = p.sb + (int64_t)(min(n0 + 16 * f, p.N - 1) / F8B) * p.Kb;
-  }
-  f32x4 acc[NF][MF];
-#pragma unroll
-  for (int f = 0; f < NF; ++f)
-#pragma unroll
-    for (int i = 0; i < MF; ++i) acc[f][i] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < MF; ++i) acc[i] = {0.f, 0.f, 0.f, 0.f};
   for (int kbase = kb0 + wave; kbase < kb1; kbase += SW * U) {
-    i32x8 b8[U][NF], a8[U][Q ? MF : 1];
-    raw32<T> av[U][Q ? 1 : MF];
-    float sb[U][NF], sa[U][MF];
+    i32x8 b8[U], a8[U][Q ? MF : 1];
+    float sb[U], sa[U][MF];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       // (a block past the end is read as the last one and takes no part)
       const int kb = min(kbase + u * SW, kb1 - 1);
+      const i32x4* s = reinterpret_cast<const i32x4*>(bp + (int64_t)kb * F8B);
+      b8[u] = cat8(s[0], s[1]);
+      sb[u] = sbp[kb];
+      if constexpr (Q)
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        const i32x4* s = reinterpret_cast<const i32x4*>(bp[f] + (int64_t)kb * F8B);
-        b8[u][f] = cat8(s[0], s[1]);
-        sb[u][f] = sbp[f][kb];
-      }
-#pragma unroll
-      for (int i = 0; i < MF; ++i) {
-        const int mc = min(m0 + 16 * i + l16, p.M - 1);
-        if constexpr (Q) {
-          const i32x4* s = reinterpret_cast<const i32x4*>((const uint8_t*)p.a + mc * Kp + (int64_t)kb * F8B + g * 32);
-          a8[u][i] = cat8(s[0], s[1]);
+        for (int i = 0; i < MF; ++i) {
+          const int mc = min(16 * i + l16, p.M - 1);
+          const i32x4* t = reinterpret_cast<const i32x4*>((const uint8_t*)p.a + mc * Kp + (int64_t)kb * F8B + g * 32);
+          a8[u][i] = cat8(t[0], t[1]);
           sa[u][i] = p.sa[(int64_t)kb * p.M + mc];
-        } else {
-          const int k = kb * F8B + g * 32;
-          av[u][i] = load32<T, VEC>((const T*)p.a + mc * p.lda + k, p.K - k);
         }
+    }
+    if constexpr (!Q) {
+      const int k = min(kbase + g * SW, kb1 - 1) * F8B + l16 * 8;
+      const T* x = (const T*)p.a + k;
+#pragma unroll 2
+      for (int m = 0; m < p.M; ++m) {
+        float v[8], sc, inv;
+        f8_load8<VEC>(x + m * p.lda, p.K - k, v);
+        uint32_t t = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t = max(t, f8_abs_bits(v[j]));
+        f8_scale<PGV_F8_E4M3>(f8_max16(t), sc, inv);
+        i32x2 o;
+        o.x = f8_pack4<PGV_F8_E4M3>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+        o.y = f8_pack4<PGV_F8_E4M3>(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+        *reinterpret_cast<i32x2*>(img + (g * 16 + m) * ROW + l16 * 8) = o;
+        if (l16 == 0) img_s[g * 16 + m] = sc;
       }
+      wave_sync();
+      // (lanes of rows that are none read whatever the image holds: their columns of the product are not stored)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const i32x4* t = reinterpret_cast<const i32x4*>(img + (u * 16 + l16) * ROW + g * 32);
+        a8[u][0] = cat8(t[0], t[1]);
+        sa[u][0] = img_s[u * 16 + l16];
+      }
+      wave_sync();   // (the next blocks go into the same image)
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (kbase + u * SW >= kb1) break;
-      frag<F32> bf[NF];
-#pragma unroll
-      for (int f = 0; f < NF; ++f) bf[f] = make_frag<PGV_F8_E4M3, F32>(b8[u][f]);
+      const frag<F32> bf = make_frag<PGV_F8_E4M3, F32>(b8[u]);
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
-        frag<F32> af;
-        if constexpr (Q)
-          af = make_frag<FA, F32>(a8[u][i]);
-        else
-          af = make_frag<PGV_F8_E4M3, F32>(quant_frag(av[u][i], sa[u][i]));
+        const f32x4 d = mfma128<FA, F32>(bf, make_frag<FA, F32>(a8[u][i]));
+        const float s = sa[u][i] * sb[u];
 #pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          const f32x4 d = mfma128<FA, F32>(bf[f], af);
-          const float s = sa[u][i] * sb[u][f];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[f][i][j] = fmaf(d[j], s, acc[f][i][j]);
-        }
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d[j], s, acc[i][j]);
       }
     }
   }
-  // the waves' sums meet, GRP tiles at a time: image [wave][tile][m 16][n 16]
+  // the waves' sums meet: image [wave][tile][m 16][n 16]
+  if constexpr (!Q) __syncthreads();   // (over the exchange images)
+  float* sum = reinterpret_cast<float*>(lds);
 #pragma unroll
-  for (int t0 = 0; t0 < NF * MF; t0 += GRP) {
-    if (t0) __syncthreads();
+  for (int i = 0; i < MF; ++i) *reinterpret_cast<f32x4*>(&sum[((wave * MF + i) * 16 + l16) * 16 + 4 * g]) = acc[i];
+  __syncthreads();
+  for (int e = tid; e < MF * 256; e += 64 * SW) {
+    const int m = e >> 4, n = n0 + (e & 15);
+    if (m >= p.M || n >= p.N) continue;
+    float s = 0.f;
 #pragma unroll
-    for (int t = 0; t < GRP; ++t) {
-      const int f = (t0 + t) / MF, i = (t0 + t) % MF;
-      if (t0 + t < NF * MF) *reinterpret_cast<f32x4*>(&lds[((wave * GRP + t) * 16 + l16) * 16 + 4 * g]) = acc[f][i];
-    }
-    __syncthreads();
-    for (int e = tid; e < GRP * 256; e += 64 * SW) {
-      const int t = e >> 8, f = (t0 + t) / MF, i = (t0 + t) % MF;
-      const int m = m0 + 16 * i + ((e >> 4) & 15), n = n0 + 16 * f + (e & 15);
-      if (t0 + t < NF * MF && m < p.M && n < p.N) {
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < SW; ++w) s += lds[w * GRP * 256 + e];
-        const int64_t o = (int64_t)m * p.N + n;
-        if (p.splits > 1)
-          p.part[(int64_t)split * p.M * p.N + o] = s;
-        else
-          f8_store(p.out, p.out_dt, o, s + (p.bias ? p.bias[n] : 0.f));
-      }
-    }
+    for (int w = 0; w < SW; ++w) s += sum[w * MF * 256 + e];
+    const int64_t o = (int64_t)m * p.N + n;
+    if (p.splits > 1)
+      p.part[(int64_t)split * p.M * p.N + o] = s;
+    else
+      f8_store(p.out, p.out_dt, o, s + (p.bias ? p.bias[n] : 0.f));
   }
 }
 
@@ -254,17 +224,25 @@ __device__ __forceinline__ i32x4 make_rsrc(const void* p, uint32_t bytes) {
   return r;
 }
 
-// 1 KB from memory into LDS: 64 lanes x 16 bytes, destination m0 + 16 * lane.  Inline asm: the compiler orders every later LDS
-// read behind the builtin's load with vmcnt(0), which would serialise the stage in flight with the stage being multiplied; the
-// kernel waits by hand before the barrier that publishes a stage.  No register is written.
+// From memory into LDS, 16 or 4 bytes per lane: destination m0 + 16 (4) * lane.  Inline asm: the compiler orders every later
+// LDS read behind the builtin's load with vmcnt(0), which would serialise the stages in flight with the stage being
+// multiplied; the kernel counts its own loads (they are the only vector memory operations of the loop) and waits by hand before
+// the barrier that publishes a stage.  No register is written.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void dma_1k(i32x4 rsrc, unsigned lds, unsigned voff, unsigned soff) {
+__device__ __forceinline__ void dma_16(i32x4 rsrc, unsigned lds, unsigned voff, unsigned soff) {
   asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
                : "memory", "m0");
 }
+__device__ __forceinline__ void dma_4(i32x4 rsrc, unsigned lds, unsigned voff) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
+}
 #pragma clang diagnostic pop
-__device__ __forceinline__ void dma_wait_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void vm_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 struct tile_args {
   int M, N, Kb, splits, tiles_m, tiles_n;
@@ -278,99 +256,122 @@ struct tile_args {
   float* part;
 };
 
-// A stage in LDS is rows of 128 bytes; the 16-byte piece c of row r sits at piece c ^ (r & 7), so that the eight rows of a
-// fragment read (same c) fall into different banks.  LDS-DMA writes lane by lane, so the permutation is applied to the
-// address each lane fetches from.
-template <int BM, int BN, int WM, int WN, bool BROW, int FA, bool F32>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void tile_kernel(tile_args p) {
+// Which tile a workgroup takes.  Consecutive workgroups go to the eight XCDs in turn, and each XCD has an L2 of its own: an XCD
+// gets a contiguous run of tiles, in bands of 4 tile columns (n) and down the rows (m) within a band, so that the 32 tiles it
+// works on at a time share 8 panels of a and 4 of b.
+__device__ __forceinline__ void tile_of(const tile_args& p, int wg, int& tm, int& tn) {
+  const int total = p.tiles_m * p.tiles_n, per = total >> 3, extra = total & 7, xcd = wg & 7, idx = wg >> 3;
+  const int t = xcd * per + min(xcd, extra) + idx;   // (workgroup wg exists only if idx < per + (xcd < extra))
+  const int band = 4 * p.tiles_m, b = t / band, r = t - b * band, width = min(4, p.tiles_n - 4 * b);
+  tm = r / width;
+  tn = 4 * b + (r - tm * width);
+}
+
+// A stage in LDS is rows of 128 bytes (BM of a, BN of b), then 256 bytes of scales per wave.  The 16-byte piece c of row r sits
+// at piece c ^ (r & 7), so that the eight rows of a fragment read (same c) fall into different banks; LDS-DMA writes lane by
+// lane, so the permutation is applied to the address each lane fetches from.  S stages: S - 1 are in flight or complete while
+// one is multiplied.  Every wave issues PW + 1 loads per stage: its pieces of 8 rows, and one of the scales.
+template <int BM, int BN, int WM, int WN, int S, bool BROW, int FA, bool F32>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) == 4 ? 2 : 1) void tile_kernel(tile_args p) {
   constexpr int NWN = BN / WN, NW = (BM / WM) * NWN, MF = WM / 16, NF = WN / 16;
-  constexpr int STAGE = (BM + BN) * F8B, PIECES = (BM + BN) / 8;
-  static_assert(PIECES % NW == 0 && (BM / 8) % (PIECES / NW) == 0, "a wave fills pieces of one operand only");
+  constexpr int ROWS = (BM + BN) * F8B, STAGE = ROWS + NW * 256, PIECES = (BM + BN) / 8, PW = PIECES / NW;
+  static_assert(PIECES % NW == 0, "every wave fills as many pieces");
+  static_assert(BM / 64 + BN / 64 <= NW && BN % 64 == 0 && WN <= F8B && F8B % WN == 0, "one load of scales per wave");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds8[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  const int tile = blockIdx.x, split = blockIdx.y;
-  const int m0 = (tile % p.tiles_m) * BM, n0 = (tile / p.tiles_m) * BN;
+  const int split = blockIdx.y;
+  int tm, tn;
+  tile_of(p, blockIdx.x, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BN;
   const int wm = (wave / NWN) * WM, wn = (wave % NWN) * WN;
   const int kb0 = (int)((int64_t)p.Kb * split / p.splits), kb1 = (int)((int64_t)p.Kb * (split + 1) / p.splits);
   const uint32_t Kp = (uint32_t)p.Kb * F8B;
-  // this wave's share of a stage: pieces of 8 rows
-  constexpr int PW = PIECES / NW;
-  const bool fills_a = wave * PW < BM / 8;
-  const int piece0 = fills_a ? wave * PW : wave * PW - BM / 8;
   const int rows_a = min(BM, p.M - m0), rows_b = min(BN, p.N - n0);
-  const i32x4 rsrc = fills_a ? make_rsrc(p.a + (int64_t)m0 * Kp, rows_a * Kp) : make_rsrc(p.b + (int64_t)n0 * Kp, rows_b * Kp);
+  const i32x4 rsrc_a = make_rsrc(p.a + (int64_t)m0 * Kp, rows_a * Kp), rsrc_b = make_rsrc(p.b + (int64_t)n0 * Kp, rows_b * Kp);
   // (the row is in the checked part of the address: a row beyond the matrix is beyond the descriptor by itself, whatever K)
   unsigned voff[PW];
 #pragma unroll
-  for (int j = 0; j < PW; ++j)
-    voff[j] = ((unsigned)(piece0 + j) * 8u + (unsigned)(lane >> 3)) * Kp + (unsigned)(((lane & 7) ^ (lane >> 3)) * 16);
-  const unsigned dst0 = lds_addr(lds8) + (unsigned)(wave * PW) * 1024u;
+  for (int j = 0; j < PW; ++j) {
+    const int piece = wave * PW + j;
+    voff[j] = ((unsigned)(piece < BM / 8 ? piece : piece - BM / 8) * 8u + (unsigned)(lane >> 3)) * Kp +
+              (unsigned)(((lane & 7) ^ (lane >> 3)) * 16);
+  }
+  // scales: waves 0 .. BM/64 - 1 fetch sa of 64 rows each, the following ones sb of 64 rows each (or the tiles' sb, one lane
+  // each); waves with neither fetch nothing (an empty descriptor), so that all count alike
+  const float* sp;
+  int sstep, svalid;
+  unsigned svoff = (unsigned)lane * 4u;
+  if (wave < BM / 64) {
+    sp = p.sa + (int64_t)kb0 * p.M + m0 + wave * 64;
+    sstep = p.M;
+    svalid = min(64, max(0, p.M - m0 - wave * 64)) * 4;
+  } else if (BROW) {
+    const int w = wave - BM / 64;
+    sp = p.sb + (int64_t)kb0 * p.N + n0 + w * 64;
+    sstep = p.N;
+    svalid = w < BN / 64 ? min(64, max(0, p.N - n0 - w * 64)) * 4 : 0;
+  } else {
+    constexpr int T = BN > F8B ? BN / F8B : 1;
+    sp = p.sb + (int64_t)(n0 / F8B) * p.Kb + kb0;
+    sstep = 1;
+    const int have = min(T, (p.N - n0 + F8B - 1) / F8B);
+    svalid = wave == BM / 64 ? ((have - 1) * p.Kb + 1) * 4 : 0;
+    svoff = lane < have ? (unsigned)lane * (unsigned)p.Kb * 4u : 0xfffffff0u;
+  }
+  const unsigned lds0 = lds_addr(lds8);
   auto fill = [&](int kb, int stage) {
+    const unsigned base = lds0 + (unsigned)stage * STAGE;
 #pragma unroll
     for (int j = 0; j < PW; ++j)
-      dma_1k(rsrc, dst0 + stage * STAGE + j * 1024u, voff[j], (unsigned)kb * F8B);
+      dma_16(wave * PW + j < BM / 8 ? rsrc_a : rsrc_b, base + (unsigned)(wave * PW + j) * 1024u, voff[j], (unsigned)kb * F8B);
+    dma_4(make_rsrc(sp + (int64_t)(kb - kb0) * sstep, (uint32_t)svalid), base + ROWS + (unsigned)wave * 256u, svoff);
   };
-  // scales: sa one float per lane and column tile; sb one per wave (tiles) or four per lane and row tile (rows)
-  const float* sap[MF];
-#pragma unroll
-  for (int i = 0; i < MF; ++i) sap[i] = p.sa + min(m0 + wm + 16 * i + l16, p.M - 1);
   f32x4 acc[NF][MF];
 #pragma unroll
   for (int f = 0; f < NF; ++f)
 #pragma unroll
     for (int i = 0; i < MF; ++i) acc[f][i] = {0.f, 0.f, 0.f, 0.f};
-  float sav[MF], sbt = 0.f, sbr[BROW ? NF : 1][4];
-  auto scales = [&](int kb) {
 #pragma unroll
-    for (int i = 0; i < MF; ++i) sav[i] = sap[i][(int64_t)kb * p.M];
-    if constexpr (BROW) {
-#pragma unroll
-      for (int f = 0; f < NF; ++f)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sbr[f][j] = p.sb[(int64_t)kb * p.N + min(n0 + wn + 16 * f + 4 * g + j, p.N - 1)];
-    } else {
-      sbt = p.sb[(int64_t)(min(n0 + wn, p.N - 1) / F8B) * p.Kb + kb];
-    }
-  };
-  if (kb0 < kb1) {
-    fill(kb0, 0);
-    dma_wait_all();
-  }
-  __syncthreads();
+  for (int s = 0; s < S - 1; ++s)
+    if (kb0 + s < kb1) fill(kb0 + s, s);
+  int stage = 0;
   for (int kb = kb0; kb < kb1; ++kb) {
-    const int stage = (kb - kb0) & 1;
-    scales(kb);
-    if (kb + 1 < kb1) fill(kb + 1, stage ^ 1);
+    if (kb + S - 2 < kb1)
+      vm_wait<(S - 2) * (PW + 1)>();
+    else
+      vm_wait<0>();
+    lds_barrier();   // stage kb is complete, and nobody reads stage kb - 1 any more
+    if (kb + S - 1 < kb1) fill(kb + S - 1, stage == 0 ? S - 1 : stage - 1);
     const uint8_t* A = lds8 + stage * STAGE;
     const uint8_t* B = A + BM * F8B;
+    const float* sA = reinterpret_cast<const float*>(A + ROWS) + wm + l16;
+    const float* sB = reinterpret_cast<const float*>(A + ROWS) + BM;
     frag<F32> bf[NF];
+    f32x4 sbr[BROW ? NF : 1];
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       const uint8_t* row = B + (wn + 16 * f + l16) * F8B;
       bf[f] = make_frag<PGV_F8_E4M3, F32>(cat8(*reinterpret_cast<const i32x4*>(row + ((2 * g) ^ (l16 & 7)) * 16),
                                                *reinterpret_cast<const i32x4*>(row + ((2 * g + 1) ^ (l16 & 7)) * 16)));
+      if constexpr (BROW) sbr[f] = *reinterpret_cast<const f32x4*>(sB + wn + 16 * f + 4 * g);
     }
+    const float sbt = BROW ? 1.f : sB[wn / F8B];
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
       const uint8_t* row = A + (wm + 16 * i + l16) * F8B;
       const frag<F32> af = make_frag<FA, F32>(cat8(*reinterpret_cast<const i32x4*>(row + ((2 * g) ^ (l16 & 7)) * 16),
                                                    *reinterpret_cast<const i32x4*>(row + ((2 * g + 1) ^ (l16 & 7)) * 16)));
+      const float s = sA[16 * i] * sbt;
+      f32x4 d[NF];
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        const f32x4 d = mfma128<FA, F32>(bf[f], af);
-        if constexpr (BROW) {
+      for (int f = 0; f < NF; ++f) d[f] = mfma128<FA, F32>(bf[f], af);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[f][i][j] = fmaf(d[j], sav[i] * sbr[f][j], acc[f][i][j]);
-        } else {
-          const float s = sav[i] * sbt;
+      for (int f = 0; f < NF; ++f)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[f][i][j] = fmaf(d[j], s, acc[f][i][j]);
-        }
-      }
+        for (int j = 0; j < 4; ++j) acc[f][i][j] = fmaf(d[f][j], BROW ? s * sbr[BROW ? f : 0][j] : s, acc[f][i][j]);
     }
-    dma_wait_all();
-    __syncthreads();
+    stage = stage + 1 == S ? 0 : stage + 1;
   }
   const bool quad = (p.N & 3) == 0;
 #pragma unroll
@@ -398,50 +399,57 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void tile_kernel(tile_a
   }
 }
 
-template <int BM, int BN, int WM, int WN, bool BROW, int FA, bool F32>
+template <int BM, int BN, int WM, int WN, int S, bool BROW, int FA, bool F32>
 int launch_tile(tile_args p, hipStream_t st) {
   p.tiles_m = (int)pgv_cdiv(p.M, BM);
   p.tiles_n = (int)pgv_cdiv(p.N, BN);
-  constexpr int lds = 2 * (BM + BN) * F8B;
-  auto k = tile_kernel<BM, BN, WM, WN, BROW, FA, F32>;
+  constexpr int threads = (BM / WM) * (BN / WN) * 64, lds = S * ((BM + BN) * F8B + threads * 4);
+  auto k = tile_kernel<BM, BN, WM, WN, S, BROW, FA, F32>;
   static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (once != hipSuccess) {
     pgv_set_error("pgv_f8_matmul: %d bytes of LDS refused: %s", lds, hipGetErrorString(once));
     return PGV_E_LAUNCH;
   }
-  k<<<dim3((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits), (BM / WM) * (BN / WN) * 64, lds, st>>>(p);
+  k<<<dim3((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits), threads, lds, st>>>(p);
   return PGV_OK;
 }
 
-template <typename T, int FA, bool F32, bool VEC, int MF, int NF, int U>
+template <typename T, int FA, bool F32, bool VEC, int MF, int U>
 void launch_skinny(const skinny_args& p, hipStream_t st) {
-  skinny_kernel<T, FA, F32, VEC, MF, NF, U>
-      <<<dim3((unsigned)pgv_cdiv(p.N, 16 * NF), (unsigned)pgv_cdiv(p.M, 16 * MF), (unsigned)p.splits), 64 * SW, 0, st>>>(p);
+  skinny_kernel<T, FA, F32, VEC, MF, U><<<dim3((unsigned)pgv_cdiv(p.N, 16), 1, (unsigned)p.splits), 64 * SW, 0, st>>>(p);
 }
 
 // ---- which kernel, and how the reduction is split: a function of the sizes alone -------------------------------------------
 struct plan {
   bool skinny;
-  int mf, nf;       // skinny
+  int mf;      // skinny: tiles of 16 rows
+  int tile;    // tile: 256, 128 or 64 rows and columns
   int splits;
 };
 
+// Tile sizes (8 waves of 128 x 64, 8 of 32 x 64, 4 of 32 x 32): the larger ones read their operands less often and are faster
+// per workgroup slot - 4096 cubed into bfloat16: 73 / 83 / 130 us - but fill the device later - 2048 cubed: 38 / 19 / 24 us,
+// 1024 x 1024 x 8192: 110 / 50 / 28 us - and a lone workgroup per CU does not hide its first and last blocks - 1024 x 25024 x 256
+// into float32: 41 / 33 / 47 us.  256: one workgroup per CU, 3.5 times the work of a 128 one at its rate; 128 and 64:
+// two per CU.
+// Splits of the reduction: only while workgroups are missing, and with 24 blocks at least each - a join costs 4 us and its
+// reads (256 x 1024 x 25024 into float32: 124 us unsplit, 31 us with 8 splits; 100 x 4096 x 4096: 15.8 us unsplit, 15.6 with 2).
 plan make_plan(int64_t M, int64_t N, int64_t Kb, int b_block) {
   plan q = {};
   q.skinny = M <= 64 && b_block == PGV_F8_TILES;
-  int64_t wgs;
-  int64_t most;
+  int64_t wgs, most;
   if (q.skinny) {
-    q.mf = M <= 16 ? 1 : M <= 32 ? 2 : M <= 48 ? 3 : 4;
-    q.nf = 1;
-    wgs = pgv_cdiv(N, 16 * q.nf);
+    q.mf = (int)pgv_cdiv(M, 16);
+    wgs = pgv_cdiv(N, 16);
     most = Kb / (2 * SW);
   } else {
-    wgs = pgv_cdiv(M, 128) * pgv_cdiv(N, 128);
-    most = Kb / 4;
+    const int64_t t256 = pgv_cdiv(M, 256) * pgv_cdiv(N, 256), t128 = pgv_cdiv(M, 128) * pgv_cdiv(N, 128);
+    q.tile = t128 < 256 ? 64 : Kb >= 8 && 7 * pgv_cdiv(t256, 256) <= 4 * pgv_cdiv(t128, 512) ? 256 : 128;
+    wgs = pgv_cdiv(M, q.tile) * pgv_cdiv(N, q.tile);
+    most = Kb / 24;
   }
-  int64_t s = wgs >= 256 ? 1 : 512 / wgs;
-  q.splits = (int)(s < 1 ? 1 : s > most ? (most < 1 ? 1 : most) : s);
+  const int64_t s = wgs >= 256 ? 1 : 512 / wgs;
+  q.splits = (int)(s < 1 || most < 1 ? 1 : s > most ? most : s);
   return q;
 }
 
@@ -466,16 +474,18 @@ int run_matmul(int64_t M, int64_t N, int64_t K, const void* a, const float* sa, 
   if (pl.skinny) {
     skinny_args p = {(int)M, (int)N, (int)K, Kb, pl.splits, a, 0, sa, (const uint8_t*)b, sb, bias, out, out_dt, part};
     if (pl.mf == 1)
-      launch_skinny<uint8_t, FA, F32, true, 1, 1, 4>(p, st);
+      launch_skinny<uint8_t, FA, F32, true, 1, 4>(p, st);
     else if (pl.mf == 2)
-      launch_skinny<uint8_t, FA, F32, true, 2, 1, 4>(p, st);
+      launch_skinny<uint8_t, FA, F32, true, 2, 4>(p, st);
     else if (pl.mf == 3)
-      launch_skinny<uint8_t, FA, F32, true, 3, 1, 3>(p, st);
+      launch_skinny<uint8_t, FA, F32, true, 3, 3>(p, st);
     else
-      launch_skinny<uint8_t, FA, F32, true, 4, 1, 2>(p, st);
+      launch_skinny<uint8_t, FA, F32, true, 4, 2>(p, st);
   } else {
     tile_args p = {(int)M, (int)N, Kb, pl.splits, 0, 0, (const uint8_t*)a, sa, (const uint8_t*)b, sb, bias, out, out_dt, part};
-    const int rc = b_block == PGV_F8_ROWS ? launch_tile<128, 128, 64, 64, true, FA, F32>(p, st) : launch_tile<128, 128, 64, 64, false, FA, F32>(p, st);
+#define PGV_TL(...) (b_block == PGV_F8_ROWS ? launch_tile<__VA_ARGS__, true, FA, F32>(p, st) : launch_tile<__VA_ARGS__, false, FA, F32>(p, st))
+    const int rc = pl.tile == 256 ? PGV_TL(256, 256, 128, 64, 2) : pl.tile == 128 ? PGV_TL(128, 128, 32, 64, 2) : PGV_TL(64, 64, 32, 32, 4);
+#undef PGV_TL
     if (rc != PGV_OK) return rc;
   }
   run_join(pl, M, N, part, bias, out, out_dt, st);
@@ -545,8 +555,7 @@ extern "C" int pgv_f8_linear(const void* x, int dtype, int64_t M, int64_t K, int
   hipStream_t st = pgv_stream(stream);
   skinny_args p = {(int)M, (int)N, (int)K, Kb, pl.splits, x, ldx, nullptr, (const uint8_t*)b, b_scale, bias, out, out_dtype, (float*)workspace};
   const bool vec = (uintptr_t)x % 16 == 0 && (ldx * f8_dt_size(dtype)) % 16 == 0;
-#define PGV_SK2(T, F32) \
-  (vec ? launch_skinny<T, 0, F32, true, 1, 1, sizeof(T) == 4 ? 2 : 4>(p, st) : launch_skinny<T, 0, F32, false, 1, 1, 1>(p, st))
+#define PGV_SK2(T, F32) (vec ? launch_skinny<T, 0, F32, true, 1, 4>(p, st) : launch_skinny<T, 0, F32, false, 1, 4>(p, st))
 #define PGV_SK(T) (out_dtype == PGV_DT_F32 ? PGV_SK2(T, true) : PGV_SK2(T, false))
   if (dtype == PGV_DT_F32)
     PGV_SK(float);

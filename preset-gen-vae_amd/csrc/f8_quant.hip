@@ -164,14 +164,21 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(const T* __restrict__ x
   }
 }
 
-// column sums from the per-tile partial sums, in the order of the tiles
+// column sums from the per-tile partial sums: 32 columns x 8 interleaved chains of tiles, then their sum
 __global__ __launch_bounds__(256) void colsum_parts_kernel(const float* __restrict__ part, int Rb, int C,
                                                            float* __restrict__ out) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= C) return;
+  __shared__ double red[8][32];
+  const int l = threadIdx.x & 31, ph = threadIdx.x >> 5, c = blockIdx.x * 32 + l;
   double t = 0.0;
-  for (int r = 0; r < Rb; ++r) t += (double)part[(int64_t)r * C + c];
-  out[c] = (float)t;
+  if (c < C)
+#pragma unroll 4
+    for (int r = ph; r < Rb; r += 8) t += (double)part[(int64_t)r * C + c];
+  red[ph][l] = t;
+  __syncthreads();
+  if (threadIdx.x < 32 && c < C) {
+    for (int i = 1; i < 8; ++i) t += red[i][l];
+    out[c] = (float)t;
+  }
 }
 
 template <typename T, int FMT>
@@ -194,7 +201,7 @@ int launch(const T* x, int64_t R, int64_t C, int64_t ldx, int block, uint8_t* q,
     else
       vec ? PGV_TILE(false, true) : PGV_TILE(false, false);
 #undef PGV_TILE
-    if (colsum) colsum_parts_kernel<<<dim3((unsigned)pgv_cdiv(C, 256)), 256, 0, st>>>(part, Rb, (int)C, colsum);
+    if (colsum) colsum_parts_kernel<<<dim3((unsigned)pgv_cdiv(C, 32)), 256, 0, st>>>(part, Rb, (int)C, colsum);
   }
   PGV_CHECK_LAUNCH("pgv_f8_quantize");
   return PGV_OK;
