@@ -452,10 +452,12 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(gn_args p) {
   chan<SAME> ch;
   load_stats(p, q, item, 0, ch);
   load_affine<VEC>(p, q, ch);
+  // (downwards: the end of a slice, which the pass before read last, is still in the last-level cache)
+  const int top = r0 + r1 - 1;
   auto get = [&](int r) {
     raw8<T> d;
     if (!Q || q.n > 0)
-      d = load_raw<VEC>(x + (int64_t)r * p.C, q.n);
+      d = load_raw<VEC>(x + (int64_t)(top - r) * p.C, q.n);
     else
       d.clear();
     return d;
@@ -466,9 +468,9 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(gn_args p) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) d[k] = get(r + k * q.rpp);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) put<VEC, Q, FMT>(p, q, ch, (int64_t)item * p.P + r + k * q.rpp, d[k]);
+    for (int k = 0; k < 4; ++k) put<VEC, Q, FMT>(p, q, ch, (int64_t)item * p.P + top - r - k * q.rpp, d[k]);
   }
-  for (; r < r1; r += q.rpp) put<VEC, Q, FMT>(p, q, ch, (int64_t)item * p.P + r, get(r));
+  for (; r < r1; r += q.rpp) put<VEC, Q, FMT>(p, q, ch, (int64_t)item * p.P + top - r, get(r));
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
@@ -723,7 +725,7 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(gn_args p) {
     c2[i] = p.coef[2 * g + 1];
   }
 #pragma unroll 2
-  for (int r = r0 + q.r; r < r1; r += q.rpp) {
+  for (int r = r1 - 1 - q.r; r >= r0; r -= q.rpp) {   // (downwards, as in gn_apply_kernel)
     const raw8<T> d = load_raw<VEC>(x + (int64_t)r * p.C, q.n), e = load_raw<VEC>(gy + (int64_t)r * p.C, q.n);
     put_gx<VEC>(p, q, ch, c1, c2, (int64_t)item * p.P + r, d, e);
   }
