@@ -28,7 +28,7 @@ struct gn_args {
   const void* gy;       // backward
   void* gx;
   float* part;          // partial sums (see each kernel)
-  float* coef;          // backward: [N][G][2] = mean(h), mean(h xh)
+  int parts;            // two-pass forward: partial sums per (item, group) that the second pass adds up itself (0: finalised)
   int W, tpr, slices;   // channels per workgroup, threads per row, pixel slices
   uint32_t m_tpr, m_cg, m_per;   // fused kernels: magic numbers of tpr, cg and the pieces (or channels) of a group in a row
   int lg;                        // log2 of the lanes that add up one group
@@ -270,7 +270,8 @@ struct sum2 {
   }
 };
 
-constexpr int MAXG = 256;   // groups of a workgroup of the fused kernels
+constexpr int MAXG = 256;    // groups of a workgroup of the fused kernels
+constexpr int MAXW = 2048;   // channels of a workgroup of the two-pass kernels: 8 for each of 256 threads
 
 // ---- forward, fused: grid (column blocks of W channels, items) -----------------------------------------------------------
 // A thread holds KV pieces in registers and KL more in LDS (16 bytes each: 16-bit types only).
@@ -425,32 +426,54 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(gn_args p) {
       [&](int g, const sum2<double>& v) { out[g] = v; });
 }
 
+__device__ __forceinline__ void finalize(const gn_args& p, const sum2<double>& v, float& mean, float& rstd) {
+  const double n = (double)p.P * (double)p.cg, m = v.a / n, var = v.b / n - m * m;
+  mean = (float)m;
+  rstd = (float)(1.0 / sqrt((var > 0.0 || var != var ? var : 0.0) + (double)p.eps));
+}
 __global__ __launch_bounds__(64) void gn_finalize_kernel(gn_args p, int parts) {
   const int g = blockIdx.x, item = blockIdx.y, lane = threadIdx.x;
   const sum2<double>* in = (const sum2<double>*)p.part + (int64_t)item * parts * p.G + g;
-  double a = 0.0, b = 0.0;
-  for (int e = lane; e < parts; e += 64) {
-    a += in[(int64_t)e * p.G].a;
-    b += in[(int64_t)e * p.G].b;
-  }
-  a = pgv_wave_sum_d(a);
-  b = pgv_wave_sum_d(b);
-  if (lane == 0) {
-    const double n = (double)p.P * (double)p.cg, m = a / n, var = b / n - m * m;
-    p.mean[(int64_t)item * p.G + g] = (float)m;
-    p.rstd[(int64_t)item * p.G + g] = (float)(1.0 / sqrt((var > 0.0 || var != var ? var : 0.0) + (double)p.eps));
-  }
+  sum2<double> v{};
+  for (int e = lane; e < parts; e += 64) v.add(in[(int64_t)e * p.G]);
+  v.a = pgv_wave_sum_d(v.a);
+  v.b = pgv_wave_sum_d(v.b);
+  const int64_t o = (int64_t)item * p.G + g;
+  if (lane == 0) finalize(p, v, p.mean[o], p.rstd[o]);
 }
 
 template <typename T, bool VEC, bool Q, int FMT, bool SAME>
 __global__ __launch_bounds__(256) void gn_apply_kernel(gn_args p) {
+  __shared__ float gs[2][MAXW + 2];
   const int item = blockIdx.z, slice = blockIdx.x, c0 = blockIdx.y * p.W;
   const place<SAME> q = my_place<SAME>(p, c0, 256);
+  const int gfirst = c0 / p.cg;
+  if (p.parts) {   // (uniform) few partial sums: every workgroup adds up those of its groups
+    const int groups = (min(c0 + p.W, p.C) - 1) / p.cg - gfirst + 1;
+    const sum2<double>* in = (const sum2<double>*)p.part + (int64_t)item * p.parts * p.G + gfirst;
+    sum_groups<256, sum2<double>>(groups, p.lg, [&](int g, int e) { return in[(int64_t)e * p.G + g]; }, [&](int) { return p.parts; },
+        [&](int g, const sum2<double>& v) {
+          finalize(p, v, gs[0][g], gs[1][g]);
+          if (slice == 0) {   // (two blocks that share a group write the same values)
+            p.mean[(int64_t)item * p.G + gfirst + g] = gs[0][g];
+            p.rstd[(int64_t)item * p.G + gfirst + g] = gs[1][g];
+          }
+        });
+    __syncthreads();
+  }
   if (q.r >= q.rpp || (!Q && q.n == 0)) return;
   const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
   const T* x = (const T*)p.x + (int64_t)item * p.P * p.C + q.c;
   chan<SAME> ch;
-  load_stats(p, q, item, 0, ch);
+  if (p.parts) {
+#pragma unroll
+    for (int i = 0; i < q.A; ++i) {
+      ch.mu[i] = i < q.n ? gs[0][q.g[i] - gfirst] : 0.f;
+      ch.rs[i] = i < q.n ? gs[1][q.g[i] - gfirst] : 0.f;
+    }
+  } else {
+    load_stats(p, q, item, 0, ch);
+  }
   load_affine<VEC>(p, q, ch);
   // (downwards: the end of a slice, which the pass before read last, is still in the last-level cache)
   const int top = r0 + r1 - 1;
@@ -686,29 +709,26 @@ __global__ __launch_bounds__(256) void gn_bwd_item_kernel(gn_args p, float* __re
     item_tot[((int64_t)item * 2 + (threadIdx.x >> 5)) * p.C + c] = s;
   }
 }
-// channel sums -> the group means of h and h xh: one wave per (group, item)
-__global__ __launch_bounds__(64) void gn_bwd_coef_kernel(gn_args p, const float* __restrict__ item_tot) {
-  const int g = blockIdx.x, item = blockIdx.y, lane = threadIdx.x;
-  const float* in = item_tot + (int64_t)item * 2 * p.C + g * p.cg;
-  double s1 = 0.0, s2 = 0.0;
-  for (int c = lane; c < p.cg; c += 64) {
-    const double ga = p.gamma ? (double)p.gamma[g * p.cg + c] : 1.0;
-    s1 += ga * (double)in[c];
-    s2 += ga * (double)in[p.C + c];
-  }
-  s1 = pgv_wave_sum_d(s1);
-  s2 = pgv_wave_sum_d(s2);
-  if (lane == 0) {
-    const double n = (double)p.P * (double)p.cg;
-    p.coef[((int64_t)item * p.G + g) * 2] = (float)(s1 / n);
-    p.coef[((int64_t)item * p.G + g) * 2 + 1] = (float)(s2 / n);
-  }
-}
-
 template <typename T, bool VEC, bool SAME>
-__global__ __launch_bounds__(256) void gn_bwd_apply_kernel(gn_args p) {
+__global__ __launch_bounds__(256) void gn_bwd_apply_kernel(gn_args p, const float* __restrict__ item_tot) {
+  __shared__ float gs[2][MAXW + 2];
   const int item = blockIdx.z, slice = blockIdx.x, c0 = blockIdx.y * p.W;
   const place<SAME> q = my_place<SAME>(p, c0, 256);
+  // the means of h and h xh of this block's groups, from the item's channel sums (a group may reach beyond the block)
+  const int gfirst = c0 / p.cg, groups = (min(c0 + p.W, p.C) - 1) / p.cg - gfirst + 1;
+  const float* tot = item_tot + (int64_t)item * 2 * p.C;
+  const float inv_n = 1.f / ((float)p.P * (float)p.cg);
+  sum_groups<256, sum2<float>>(groups, p.lg,
+      [&](int g, int i) {
+        const int c = (gfirst + g) * p.cg + i;
+        const float ga = p.gamma ? p.gamma[c] : 1.f;
+        sum2<float> v;
+        v.a = ga * tot[c];
+        v.b = ga * tot[p.C + c];
+        return v;
+      },
+      [&](int) { return p.cg; }, [&](int g, const sum2<float>& v) { gs[0][g] = v.a * inv_n, gs[1][g] = v.b * inv_n; });
+  __syncthreads();
   if (q.n == 0) return;
   const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
   const int64_t base = (int64_t)item * p.P * p.C + q.c;
@@ -720,9 +740,8 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(gn_args p) {
   float c1[q.A], c2[q.A];
 #pragma unroll
   for (int i = 0; i < q.A; ++i) {
-    const int64_t g = (int64_t)item * p.G + q.g[i];
-    c1[i] = p.coef[2 * g];
-    c2[i] = p.coef[2 * g + 1];
+    c1[i] = gs[0][i < q.n ? q.g[i] - gfirst : 0];
+    c2[i] = gs[1][i < q.n ? q.g[i] - gfirst : 0];
   }
 #pragma unroll 2
   for (int r = r1 - 1 - q.r; r >= r0; r -= q.rpp) {   // (downwards, as in gn_apply_kernel)
@@ -810,7 +829,7 @@ gn_plan make_gn_plan(int64_t N, int64_t P, int64_t C, int64_t G, int esize, int 
         return r;
       }
     }
-  r.W = (int)(C < 2048 ? C : 2048);
+  r.W = (int)(C < MAXW ? C : MAXW);
   r.tpr = (int)(kind == 1 ? pgv_cdiv(r.W, F8B) * 16 : pgv_cdiv(r.W, 8));
   r.colblocks = (int)pgv_cdiv(C, r.W);
   r.lg = lanes_log2(256, G);
@@ -873,7 +892,10 @@ int gn_forward(gn_args p, const gn_plan& pl, hipStream_t st) {
   }
   const dim3 grid((unsigned)pl.slices, (unsigned)pl.colblocks, (unsigned)p.N);
   gn_stats_kernel<T, VEC, SAME><<<grid, 256, 0, st>>>(p);
-  gn_finalize_kernel<<<dim3((unsigned)p.G, (unsigned)p.N), 64, 0, st>>>(p, pl.slices * pl.colblocks);
+  // (a launch costs 5 us; 32 sums of 32 groups read by every workgroup cost 1, 128 of them more than the launch)
+  const int parts = pl.slices * pl.colblocks;
+  p.parts = parts <= 32 ? parts : 0;
+  if (!p.parts) gn_finalize_kernel<<<dim3((unsigned)p.G, (unsigned)p.N), 64, 0, st>>>(p, parts);
   gn_apply_kernel<T, VEC, Q, FMT, SAME><<<grid, 256, 0, st>>>(p);
   return PGV_OK;
 }
@@ -914,11 +936,9 @@ int gn_backward(gn_args p, const gn_plan& pl, float* ggamma, float* gbeta, hipSt
   } else {
     const dim3 grid((unsigned)pl.slices, (unsigned)pl.colblocks, (unsigned)p.N);
     float* tot = p.part + (int64_t)p.N * pl.slices * 2 * p.C;
-    p.coef = tot + (int64_t)p.N * 2 * p.C;
     gn_bwd_sums_kernel<T, VEC, SAME><<<grid, 256, 0, st>>>(p);
     gn_bwd_item_kernel<<<dim3((unsigned)pgv_cdiv(p.C, 32), (unsigned)p.N), 256, 0, st>>>(p, tot);
-    gn_bwd_coef_kernel<<<dim3((unsigned)p.G, (unsigned)p.N), 64, 0, st>>>(p, tot);
-    gn_bwd_apply_kernel<T, VEC, SAME><<<grid, 256, 0, st>>>(p);
+    gn_bwd_apply_kernel<T, VEC, SAME><<<grid, 256, 0, st>>>(p, tot);
     item_tot = tot;
   }
   if (ggamma || gbeta)
@@ -931,7 +951,7 @@ int gn_backward(gn_args p, const gn_plan& pl, float* ggamma, float* gbeta, hipSt
 extern "C" int64_t pgv_group_norm_workspace(int64_t N, int64_t P, int64_t C, int64_t G, int dtype, int kind) {
   if (N <= 0 || P <= 0 || C <= 0 || G <= 0 || C % G || !f8_dt_ok(dtype) || kind < 0 || kind > 2) return 0;
   const gn_plan pl = make_gn_plan(N, P, C, G, f8_dt_size(dtype), kind);
-  if (kind == 2) return 4 * (pl.fused ? N * 2 * C : N * (pl.slices + 1) * 2 * C + N * G * 2);
+  if (kind == 2) return 4 * (pl.fused ? N * 2 * C : N * (pl.slices + 1) * 2 * C);
   const int64_t stats = kind == 1 && !pl.fused ? 8 * N * G : 0;   // mean and rstd live here when the caller has no use for them
   return stats + (pl.fused ? 0 : 16 * N * G * pl.slices * pl.colblocks);
 }

@@ -157,7 +157,9 @@ def check_product(y, a, b, bias=None):
 
 MNK = [(1, 1, 1), (1, 16, 128), (1, 130, 4100), (3, 17, 129), (16, 256, 2048), (17, 33, 640), (33, 100, 300), (64, 129, 1000),
        (65, 64, 128), (100, 1000, 72), (128, 128, 128), (129, 257, 385), (200, 72, 5000), (300, 520, 1408), (257, 1024, 2176),
-       (600, 300, 256), (1030, 520, 640)]
+       (600, 300, 256), (1030, 520, 640),
+       # the larger tiles with ragged edges, and a split reduction of the smallest
+       (2100, 2050, 300), (4090, 4093, 1100), (70, 90, 7000)]
 
 
 @pytest.mark.parametrize("mnk", MNK)

@@ -89,7 +89,9 @@ def check(ops, x, gy, G, w, b, act, eps=1e-5):
 # group, every channel a group, slabs that fit a workgroup's registers and slabs that do not, more channels than a block has columns
 SHAPES = [(1, 1, 32, 4), (1, 12, 2048, 32), (2, 391, 64, 8), (3, 17, 6, 3), (2, 33, 5, 1), (2, 40, 12, 12), (4, 1, 1024, 32),
           (2, 100, 24, 3), (1, 1485, 96, 4), (2, 5000, 32, 8), (1, 3000, 20, 5), (1, 9, 4104, 3), (1, 600, 2600, 2), (1, 70, 2304, 96),
-          (2, 700, 256, 32), (1, 4100, 512, 32), (1, 2, 16400, 2)]
+          (2, 700, 256, 32), (1, 4100, 512, 32), (1, 2, 16400, 2),
+          # one wave per workgroup (many small slabs), the largest slabs in registers, and slices of 128 partial sums
+          (1100, 5, 32, 4), (300, 40, 128, 16), (2, 1485, 256, 16), (1, 1000, 64, 2), (2, 20000, 128, 4)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -181,7 +183,8 @@ def step_of(v, fmt):
 
 
 @pytest.mark.parametrize("shape", [(1, 12, 2048, 32), (3, 20, 128, 8), (2, 33, 100, 4), (2, 50, 6, 3), (2, 3000, 256, 32), (1, 40, 2304, 12),
-                                   (1, 700, 200, 5), (64, 1, 1024, 32), (1, 2200, 384, 4)])
+                                   (1, 700, 200, 5), (64, 1, 1024, 32), (1, 2200, 384, 4), (600, 9, 256, 8), (2, 1485, 256, 16),
+                                   (1, 1400, 384, 12), (1, 1400, 130, 13)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_eight_bit_output(ops, shape, dtype):
     """Scales to float32 accuracy; every byte within half a step of the scaled 64-bit result (plus the 1e-6 of the value)."""
