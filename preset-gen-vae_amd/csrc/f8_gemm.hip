@@ -432,21 +432,26 @@ struct plan {
 // 1024 x 1024 x 8192: 110 / 50 / 28 us - and a lone workgroup per CU does not hide its first and last blocks - 1024 x 25024 x 256
 // into float32: 41 / 33 / 47 us.  256: one workgroup per CU, 3.5 times the work of a 128 one at its rate; 128 and 64:
 // two per CU.
-// Splits of the reduction: only while workgroups are missing, and with 24 blocks at least each - a join costs 4 us and its
-// reads (256 x 1024 x 25024 into float32: 124 us unsplit, 31 us with 8 splits; 100 x 4096 x 4096: 15.8 us unsplit, 15.6 with 2).
+// Skinny: b is read by 16 rows at a time and a by every workgroup; from 17 rows on the 64 x 64 tiles take over where there are
+// enough of them (64 x 16384 x 4096: 18 us against 40; 64 x 4096 x 4096: 15 against 14).
+// Splits of the reduction: only while workgroups are missing, and with 12 blocks at least each - a join costs 4 us and its
+// reads (256 x 1024 x 25024 into float32: 124 us unsplit, 31 us with 8 splits; 100 x 4096 x 4096: 15.8 us unsplit, 15.6 with 2);
+// skinny from 17 instructions per wave on, with 8 each (37 x 1024 x 24576: 45 us unsplit, 16.7 with 8; 17 x 2048 x 8192: 11 us
+// unsplit, 13.5 with 2).
 plan make_plan(int64_t M, int64_t N, int64_t Kb, int b_block) {
   plan q = {};
-  q.skinny = M <= 64 && b_block == PGV_F8_TILES;
+  q.skinny = b_block == PGV_F8_TILES && (M <= 16 || (M <= 64 && N <= 8192));
   int64_t wgs, most;
   if (q.skinny) {
     q.mf = (int)pgv_cdiv(M, 16);
     wgs = pgv_cdiv(N, 16);
-    most = Kb / (2 * SW);
+    const int64_t work = pgv_cdiv(Kb, SW) * q.mf;   // instructions of a wave
+    most = work <= 16 ? 1 : pgv_cdiv(work, 8) < Kb / (2 * SW) ? pgv_cdiv(work, 8) : Kb / (2 * SW);
   } else {
     const int64_t t256 = pgv_cdiv(M, 256) * pgv_cdiv(N, 256), t128 = pgv_cdiv(M, 128) * pgv_cdiv(N, 128);
     q.tile = t128 < 256 ? 64 : Kb >= 8 && 7 * pgv_cdiv(t256, 256) <= 4 * pgv_cdiv(t128, 512) ? 256 : 128;
     wgs = pgv_cdiv(M, q.tile) * pgv_cdiv(N, q.tile);
-    most = Kb / 24;
+    most = Kb / 12;
   }
   const int64_t s = wgs >= 256 ? 1 : 512 / wgs;
   q.splits = (int)(s < 1 || most < 1 ? 1 : s > most ? most : s);
@@ -525,8 +530,9 @@ extern "C" int pgv_f8_matmul(int64_t M, int64_t N, int64_t K, const void* a, con
 #undef PGV_MM
 }
 
-// How many rows the skinny kernel quantises by itself: every workgroup repeats that work for its 16 columns.
-static constexpr int64_t FUSED_ROWS = 16;
+// How many rows the skinny kernel quantises by itself: every workgroup repeats that work for its 16 columns (8 rows x 16384 x
+// 4096: 21 us, as much as in two launches; 16 rows: 29 against 23).
+static constexpr int64_t FUSED_ROWS = 8;
 
 extern "C" int pgv_f8_linear_fused(int64_t M, int b_block) { return M <= FUSED_ROWS && b_block == PGV_F8_TILES; }
 

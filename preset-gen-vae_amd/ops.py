@@ -1013,8 +1013,11 @@ def _f8_matmul_ws(M, N, K, b_block):
 
 
 @functools.lru_cache(maxsize=4096)
-def _f8_fused(M, b_block):
-    return bool(_lib.load().pgv_f8_linear_fused(M, b_block))
+def _f8_linear_ws(M, N, K, b_block):
+    """Bytes of the quantised rows, of their scales and of the partial results of an ``fp8_linear``, each a multiple of 16."""
+    Kb = (K + 127) // 128
+    part = (_f8_matmul_ws(M, N, K, b_block) + 15) // 16 * 16
+    return (0, 0, part) if _lib.load().pgv_f8_linear_fused(M, b_block) else (M * Kb * 128, (M * Kb * 4 + 15) // 16 * 16, part)
 
 
 def _f8_out(who, like, M, N, dtype, out):
@@ -1076,13 +1079,13 @@ def fp8_linear(x, w, bias=None, out_dtype=None, out=None):
     if K == 0:
         return y.zero_() if bias is None else y.copy_(bias.expand(M, N))
     kind = F8_BLOCK_KINDS[w.block]
-    nbytes = _f8_matmul_ws(M, N, K, kind)
-    xq = None if _f8_fused(M, kind) else _f8_alloc(x, M, K, 'row', 'e4m3')
-    ws = x.new_empty(nbytes // 4, dtype=torch.float32) if nbytes else None
+    q_bytes, s_bytes, p_bytes = _f8_linear_ws(M, N, K, kind)      # one buffer: partial results, quantised rows, their scales
+    buf = x.new_empty(p_bytes + q_bytes + s_bytes, dtype=torch.uint8) if p_bytes + q_bytes else None   # (lives until the launches)
+    ws = None if buf is None else buf.data_ptr()
     _lib.check(_lib.load().pgv_f8_linear(x.data_ptr(), code, M, K, ld, w.q.data_ptr(), w.scale.data_ptr(), kind, N, _p(bias),
-                                         None if xq is None else xq.q.data_ptr(),
-                                         None if xq is None else xq.scale.data_ptr(), y.data_ptr(), _DT_CODE[y.dtype],
-                                         _p(ws), nbytes, _raw_stream(x.get_device())), "pgv_f8_linear")
+                                         ws + p_bytes if q_bytes else None, ws + p_bytes + q_bytes if q_bytes else None,
+                                         y.data_ptr(), _DT_CODE[y.dtype], ws if p_bytes else None, p_bytes,
+                                         _raw_stream(x.get_device())), "pgv_f8_linear")
     return y
 
 
