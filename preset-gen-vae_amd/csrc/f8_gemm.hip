@@ -295,7 +295,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) =
   for (int j = 0; j < PW; ++j) {
     const int piece = wave * PW + j;
     voff[j] = ((unsigned)(piece < BM / 8 ? piece : piece - BM / 8) * 8u + (unsigned)(lane >> 3)) * Kp +
-              (unsigned)(((lane & 7) ^ (lane >> 3)) * 16);
+              (unsigned)(((lane & 7) ^ (lane >> 3) ^ (piece & 1)) * 16);
   }
   // scales: waves 0 .. BM/64 - 1 fetch sa of 64 rows each, the following ones sb of 64 rows each (or the tiles' sb, one lane
   // each); waves with neither fetch nothing (an empty descriptor), so that all count alike
@@ -352,16 +352,16 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) =
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       const uint8_t* row = B + (wn + 16 * f + l16) * F8B;
-      bf[f] = make_frag<PGV_F8_E4M3, F32>(cat8(*reinterpret_cast<const i32x4*>(row + ((2 * g) ^ (l16 & 7)) * 16),
-                                               *reinterpret_cast<const i32x4*>(row + ((2 * g + 1) ^ (l16 & 7)) * 16)));
+      bf[f] = make_frag<PGV_F8_E4M3, F32>(cat8(*reinterpret_cast<const i32x4*>(row + ((2 * g) ^ (l16 & 7) ^ (l16 >> 3)) * 16),
+                                               *reinterpret_cast<const i32x4*>(row + ((2 * g + 1) ^ (l16 & 7) ^ (l16 >> 3)) * 16)));
       if constexpr (BROW) sbr[f] = *reinterpret_cast<const f32x4*>(sB + wn + 16 * f + 4 * g);
     }
     const float sbt = BROW ? 1.f : sB[wn / F8B];
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
       const uint8_t* row = A + (wm + 16 * i + l16) * F8B;
-      const frag<F32> af = make_frag<FA, F32>(cat8(*reinterpret_cast<const i32x4*>(row + ((2 * g) ^ (l16 & 7)) * 16),
-                                                   *reinterpret_cast<const i32x4*>(row + ((2 * g + 1) ^ (l16 & 7)) * 16)));
+      const frag<F32> af = make_frag<FA, F32>(cat8(*reinterpret_cast<const i32x4*>(row + ((2 * g) ^ (l16 & 7) ^ (l16 >> 3)) * 16),
+                                                   *reinterpret_cast<const i32x4*>(row + ((2 * g + 1) ^ (l16 & 7) ^ (l16 >> 3)) * 16)));
       const float s = sA[16 * i] * sbt;
       f32x4 d[NF];
 #pragma unroll
