@@ -29,7 +29,7 @@ struct gn_args {
   void* gx;
   float* part;          // partial sums (see each kernel)
   int parts;            // two-pass forward: partial sums per (item, group) that the second pass adds up itself (0: finalised)
-  int W, tpr, slices;   // channels per workgroup, threads per row, pixel slices
+  int W, tpr, slices, colblocks;   // channels per workgroup, threads per row, pixel slices of an item, column blocks of a row
   uint32_t m_tpr, m_cg, m_per;   // fused kernels: magic numbers of tpr, cg and the pieces (or channels) of a group in a row
   int lg;                        // log2 of the lanes that add up one group
 };
@@ -40,6 +40,7 @@ static inline uint32_t magic_of(int64_t d) { return d <= 1 ? 0u : (uint32_t)(((1
 
 // 1 / sqrt(v) within an ulp: the hardware's estimate and one Newton step
 __device__ __forceinline__ float rsqrt_(float v) {
+  if (v < 0x1p-100f) return 1.f / sqrtf(v);   // (the estimate takes a denormal for zero)
   const float y = __builtin_amdgcn_rsqf(v);
   return fmaf(y * 0.5f, fmaf(-v * y, y, 1.f), y);
 }
@@ -273,7 +274,7 @@ struct sum2 {
 constexpr int MAXG = 256;    // groups of a workgroup of the fused kernels
 constexpr int MAXW = 2048;   // channels of a workgroup of the two-pass kernels: 8 for each of 256 threads
 
-// ---- forward, fused: grid (column blocks of W channels, items) -----------------------------------------------------------
+// ---- forward, fused: a workgroup per item and column block of W channels -----------------------------------------------------------
 // A thread holds KV pieces in registers and KL more in LDS (16 bytes each: 16-bit types only).
 template <typename T, int NT, int KV, int KL, bool VEC, bool Q, int FMT, bool SAME>
 __global__ __launch_bounds__(NT) void gn_fwd_fused_kernel(gn_args p) {
@@ -281,9 +282,9 @@ __global__ __launch_bounds__(NT) void gn_fwd_fused_kernel(gn_args p) {
   extern __shared__ __attribute__((aligned(16))) i32x4 held[];   // [KL][NT]
   __shared__ __attribute__((aligned(16))) float val[NT * A];
   __shared__ float gs[2][MAXG];
-  const int tid = threadIdx.x, item = blockIdx.y, c0 = blockIdx.x * p.W;
+  const int tid = threadIdx.x, item = blockIdx.x / p.colblocks, cb = blockIdx.x - item * p.colblocks, c0 = cb * p.W;
   const place<SAME> q = my_place<SAME, true>(p, c0, NT);
-  const int gfirst = blockIdx.x * (p.W / p.cg), groups = min(p.W / p.cg, p.G - gfirst);
+  const int gfirst = cb * (p.W / p.cg), groups = min(p.W / p.cg, p.G - gfirst);
   const T* x = (const T*)p.x + (int64_t)item * p.P * p.C;   // (the item's bytes are addressed with 32 bits: make_gn_plan)
   const uint32_t at0 = (uint32_t)(q.r * p.C + q.c), step = (uint32_t)(q.rpp * p.C);
   auto get = [&](int k) {
@@ -388,7 +389,7 @@ template <typename T, bool VEC, bool SAME>
 __global__ __launch_bounds__(256) void gn_stats_kernel(gn_args p) {
   constexpr int A = SAME ? 1 : 8;
   __shared__ sum2<double> val[256 * A];
-  const int tid = threadIdx.x, item = blockIdx.z, slice = blockIdx.x, c0 = blockIdx.y * p.W;
+  const int tid = threadIdx.x, item = blockIdx.x / p.slices, slice = blockIdx.x - item * p.slices, c0 = blockIdx.y * p.W;
   const place<SAME> q = my_place<SAME>(p, c0, 256);
   const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
   const T* x = (const T*)p.x + (int64_t)item * p.P * p.C + q.c;
@@ -432,7 +433,7 @@ __device__ __forceinline__ void finalize(const gn_args& p, const sum2<double>& v
   rstd = (float)(1.0 / sqrt((var > 0.0 || var != var ? var : 0.0) + (double)p.eps));
 }
 __global__ __launch_bounds__(64) void gn_finalize_kernel(gn_args p, int parts) {
-  const int g = blockIdx.x, item = blockIdx.y, lane = threadIdx.x;
+  const int item = blockIdx.x / p.G, g = blockIdx.x - item * p.G, lane = threadIdx.x;
   const sum2<double>* in = (const sum2<double>*)p.part + (int64_t)item * parts * p.G + g;
   sum2<double> v{};
   for (int e = lane; e < parts; e += 64) v.add(in[(int64_t)e * p.G]);
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(64) void gn_finalize_kernel(gn_args p, int parts) {
 template <typename T, bool VEC, bool Q, int FMT, bool SAME>
 __global__ __launch_bounds__(256) void gn_apply_kernel(gn_args p) {
   __shared__ float gs[2][MAXW + 2];
-  const int item = blockIdx.z, slice = blockIdx.x, c0 = blockIdx.y * p.W;
+  const int item = blockIdx.x / p.slices, slice = blockIdx.x - item * p.slices, c0 = blockIdx.y * p.W;
   const place<SAME> q = my_place<SAME>(p, c0, 256);
   const int gfirst = c0 / p.cg;
   if (p.parts) {   // (uniform) few partial sums: every workgroup adds up those of its groups
@@ -578,9 +579,9 @@ __global__ __launch_bounds__(NT) void gn_bwd_fused_kernel(gn_args p) {
   float* val = sm;                 // [2][NT * 8]
   float* tot = sm + NT * 16;       // [2][width]
   __shared__ float gs[2][MAXG];
-  const int item = blockIdx.y, c0 = blockIdx.x * p.W, width = min(p.W, p.C - c0);
+  const int item = blockIdx.x / p.colblocks, cb = blockIdx.x - item * p.colblocks, c0 = cb * p.W, width = min(p.W, p.C - c0);
   const place<SAME> q = my_place<SAME, true>(p, c0, NT);
-  const int gfirst = blockIdx.x * (p.W / p.cg);
+  const int gfirst = cb * (p.W / p.cg);
   const T* x = (const T*)p.x + (int64_t)item * p.P * p.C;
   const T* gy = (const T*)p.gy + (int64_t)item * p.P * p.C;
   const uint32_t at0 = (uint32_t)(q.r * p.C + q.c), step = (uint32_t)(q.rpp * p.C);
@@ -648,7 +649,7 @@ template <typename T, bool VEC, bool SAME>
 __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(gn_args p) {
   __shared__ __attribute__((aligned(16))) float val[4096];
   __shared__ float tot[4096];
-  const int item = blockIdx.z, slice = blockIdx.x, c0 = blockIdx.y * p.W, width = min(p.W, p.C - c0);
+  const int item = blockIdx.x / p.slices, slice = blockIdx.x - item * p.slices, c0 = blockIdx.y * p.W, width = min(p.W, p.C - c0);
   const place<SAME> q = my_place<SAME>(p, c0, 256);
   const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
   const int64_t base = (int64_t)item * p.P * p.C + q.c;
@@ -691,7 +692,7 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(gn_args p) {
 // slices -> channel sums of the item, item_tot [N][2][C]: 32 channels x 8 interleaved chains of slices per workgroup
 __global__ __launch_bounds__(256) void gn_bwd_item_kernel(gn_args p, float* __restrict__ item_tot) {
   __shared__ float red[8][64];
-  const int l = threadIdx.x & 31, ph = threadIdx.x >> 5, c = blockIdx.x * 32 + l, item = blockIdx.y;
+  const int l = threadIdx.x & 31, ph = threadIdx.x >> 5, c = blockIdx.y * 32 + l, item = blockIdx.x;
   const float* in = p.part + (int64_t)item * p.slices * 2 * p.C + c;
   float a = 0.f, b = 0.f;
   if (c < p.C)
@@ -712,7 +713,7 @@ __global__ __launch_bounds__(256) void gn_bwd_item_kernel(gn_args p, float* __re
 template <typename T, bool VEC, bool SAME>
 __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(gn_args p, const float* __restrict__ item_tot) {
   __shared__ float gs[2][MAXW + 2];
-  const int item = blockIdx.z, slice = blockIdx.x, c0 = blockIdx.y * p.W;
+  const int item = blockIdx.x / p.slices, slice = blockIdx.x - item * p.slices, c0 = blockIdx.y * p.W;
   const place<SAME> q = my_place<SAME>(p, c0, 256);
   // the means of h and h xh of this block's groups, from the item's channel sums (a group may reach beyond the block)
   const int gfirst = c0 / p.cg, groups = (min(c0 + p.W, p.C) - 1) / p.cg - gfirst + 1;
@@ -750,15 +751,19 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(gn_args p, const floa
   }
 }
 
-// gbeta / ggamma: rows [rows][2][C] of channel sums, added in a fixed order (32 interleaved chains, then their sum)
+// gbeta / ggamma: rows [rows][2][C] of channel sums, added in a fixed order (32 interleaved chains, then their sum).  With more
+// than ROWS rows the workgroups along y take ROWS each and leave rows of the same layout in `next` for a second launch.
+constexpr int ROWS = 1024;
 __global__ __launch_bounds__(1024) void gn_param_grads_kernel(const float* __restrict__ part, int rows, int C,
-                                                              float* __restrict__ ggamma, float* __restrict__ gbeta) {
+                                                              float* __restrict__ ggamma, float* __restrict__ gbeta,
+                                                              float* __restrict__ next) {
   __shared__ double red[32][65];
-  const int l = threadIdx.x & 31, ph = threadIdx.x >> 5, c = blockIdx.x * 32 + l;
+  const int l = threadIdx.x & 31, ph = threadIdx.x >> 5, c = blockIdx.x * 32 + l, r0 = blockIdx.y * ROWS;
+  const int r1 = min(rows, r0 + ROWS);
   double a = 0.0, b = 0.0;
   if (c < C)
 #pragma unroll 4
-    for (int r = ph; r < rows; r += 32) {
+    for (int r = r0 + ph; r < r1; r += 32) {
       a += (double)part[(int64_t)r * 2 * C + c];
       b += (double)part[((int64_t)r * 2 + 1) * C + c];
     }
@@ -770,6 +775,7 @@ __global__ __launch_bounds__(1024) void gn_param_grads_kernel(const float* __res
 #pragma unroll 8
     for (int i = 0; i < 32; ++i) s += red[i][threadIdx.x];
     float* out = threadIdx.x < 32 ? gbeta : ggamma;
+    if (next) out = next + ((int64_t)blockIdx.y * 2 + (threadIdx.x >> 5)) * C;
     if (out && c < C) out[c] = (float)s;
   }
 }
@@ -801,6 +807,7 @@ gn_plan make_gn_plan(int64_t N, int64_t P, int64_t C, int64_t G, int esize, int 
   W = cg / gcd_(cg, unit) * unit;
   if (W < C && W * esize < 128) W = W * pgv_cdiv(128, W * esize);
   if (W % 8 && W < C) W = W * (8 / gcd_(W, 8));
+  while (P * pgv_cdiv(W, 8) < 64 && W < C) W *= 2;   // few pixels: enough channels for a wave
   if (W > C) W = C;
   int64_t tpr = pgv_cdiv(W, 8);
   if (kind == 1) tpr = pgv_cdiv(W, F8B) * 16;
@@ -846,7 +853,7 @@ int gn_check(const char* who, int64_t N, int64_t P, int64_t C, int64_t G, int dt
   PGV_CHECK_ARG(act >= PGV_ACT_NONE && act <= PGV_ACT_SILU, "%s: unknown activation %d", who, act);
   PGV_CHECK_ARG(N >= 0 && P >= 0 && C >= 0 && G > 0 && C % G == 0, "%s: bad sizes N=%lld P=%lld C=%lld groups=%lld", who,
                 (long long)N, (long long)P, (long long)C, (long long)G);
-  PGV_CHECK_ARG(N <= 65535 && P <= (1ll << 28) && C <= (1ll << 20), "%s: too large (items %lld, pixels %lld, channels %lld)", who,
+  PGV_CHECK_ARG(N <= (1ll << 24) && P <= (1ll << 28) && C <= (1ll << 20) && N * G < (1ll << 31), "%s: too large (items %lld, pixels %lld, channels %lld)", who,
                 (long long)N, (long long)P, (long long)C);
   return PGV_OK;
 }
@@ -855,6 +862,7 @@ void set_plan(gn_args& p, const gn_plan& pl, bool same) {
   p.W = pl.W;
   p.tpr = pl.tpr;
   p.slices = pl.slices;
+  p.colblocks = pl.colblocks;
   p.lg = pl.lg;
   p.m_tpr = magic_of(pl.tpr);
   p.m_cg = magic_of(p.cg);
@@ -865,7 +873,7 @@ template <typename T, bool VEC, bool Q, int FMT, bool SAME>
 int gn_forward(gn_args p, const gn_plan& pl, hipStream_t st) {
   set_plan(p, pl, SAME);
   if (pl.fused) {
-    const dim3 grid((unsigned)pl.colblocks, (unsigned)p.N);
+    const dim3 grid((unsigned)((int64_t)p.N * pl.colblocks));
 #define PGV_F(NT, KV) gn_fwd_fused_kernel<T, NT, KV, 0, VEC, Q, FMT, SAME><<<grid, NT, 0, st>>>(p)
     if (pl.nt == 64)
       pl.kv == 1 ? PGV_F(64, 1) : pl.kv == 4 ? PGV_F(64, 4) : PGV_F(64, 8);
@@ -890,12 +898,12 @@ int gn_forward(gn_args p, const gn_plan& pl, hipStream_t st) {
 #undef PGV_F
     return PGV_OK;
   }
-  const dim3 grid((unsigned)pl.slices, (unsigned)pl.colblocks, (unsigned)p.N);
+  const dim3 grid((unsigned)((int64_t)p.N * pl.slices), (unsigned)pl.colblocks);
   gn_stats_kernel<T, VEC, SAME><<<grid, 256, 0, st>>>(p);
   // (a launch costs 5 us; 32 sums of 32 groups read by every workgroup cost 1, 128 of them more than the launch)
   const int parts = pl.slices * pl.colblocks;
   p.parts = parts <= 32 ? parts : 0;
-  if (!p.parts) gn_finalize_kernel<<<dim3((unsigned)p.G, (unsigned)p.N), 64, 0, st>>>(p, parts);
+  if (!p.parts) gn_finalize_kernel<<<dim3((unsigned)((int64_t)p.G * p.N)), 64, 0, st>>>(p, parts);
   gn_apply_kernel<T, VEC, Q, FMT, SAME><<<grid, 256, 0, st>>>(p);
   return PGV_OK;
 }
@@ -918,7 +926,7 @@ int gn_backward(gn_args p, const gn_plan& pl, float* ggamma, float* gbeta, hipSt
   set_plan(p, pl, SAME);
   const float* item_tot = p.part;
   if (pl.fused) {
-    const dim3 grid((unsigned)pl.colblocks, (unsigned)p.N);
+    const dim3 grid((unsigned)((int64_t)p.N * pl.colblocks));
     int rc = PGV_OK;
     if (pl.nt == 64)
       rc = pl.kv == 1   ? launch_bwd_fused<T, 64, 1, VEC, SAME>(p, grid, st)
@@ -934,15 +942,26 @@ int gn_backward(gn_args p, const gn_plan& pl, float* ggamma, float* gbeta, hipSt
       rc = launch_bwd_fused<T, 512, 16, VEC, SAME>(p, grid, st);
     if (rc != PGV_OK) return rc;
   } else {
-    const dim3 grid((unsigned)pl.slices, (unsigned)pl.colblocks, (unsigned)p.N);
+    const dim3 grid((unsigned)((int64_t)p.N * pl.slices), (unsigned)pl.colblocks);
     float* tot = p.part + (int64_t)p.N * pl.slices * 2 * p.C;
     gn_bwd_sums_kernel<T, VEC, SAME><<<grid, 256, 0, st>>>(p);
-    gn_bwd_item_kernel<<<dim3((unsigned)pgv_cdiv(p.C, 32), (unsigned)p.N), 256, 0, st>>>(p, tot);
+    gn_bwd_item_kernel<<<dim3((unsigned)p.N, (unsigned)pgv_cdiv(p.C, 32)), 256, 0, st>>>(p, tot);
     gn_bwd_apply_kernel<T, VEC, SAME><<<grid, 256, 0, st>>>(p, tot);
     item_tot = tot;
   }
-  if (ggamma || gbeta)
-    gn_param_grads_kernel<<<dim3((unsigned)pgv_cdiv(p.C, 32)), 1024, 0, st>>>(item_tot, p.N, p.C, ggamma, gbeta);
+  if (ggamma || gbeta) {
+    const unsigned cols = (unsigned)pgv_cdiv(p.C, 32);
+    int rows = p.N;
+    float* next = p.part + (int64_t)p.N * (pl.fused ? 1 : pl.slices + 1) * 2 * p.C;
+    while (rows > ROWS) {
+      const int n = (int)pgv_cdiv(rows, ROWS);
+      gn_param_grads_kernel<<<dim3(cols, (unsigned)n), 1024, 0, st>>>(item_tot, rows, p.C, nullptr, nullptr, next);
+      item_tot = next;
+      next += (int64_t)n * 2 * p.C;
+      rows = n;
+    }
+    gn_param_grads_kernel<<<dim3(cols), 1024, 0, st>>>(item_tot, rows, p.C, ggamma, gbeta, nullptr);
+  }
   return PGV_OK;
 }
 
@@ -951,7 +970,11 @@ int gn_backward(gn_args p, const gn_plan& pl, float* ggamma, float* gbeta, hipSt
 extern "C" int64_t pgv_group_norm_workspace(int64_t N, int64_t P, int64_t C, int64_t G, int dtype, int kind) {
   if (N <= 0 || P <= 0 || C <= 0 || G <= 0 || C % G || !f8_dt_ok(dtype) || kind < 0 || kind > 2) return 0;
   const gn_plan pl = make_gn_plan(N, P, C, G, f8_dt_size(dtype), kind);
-  if (kind == 2) return 4 * (pl.fused ? N * 2 * C : N * (pl.slices + 1) * 2 * C);
+  if (kind == 2) {
+    int64_t rows = N * (pl.fused ? 1 : pl.slices + 1);
+    for (int64_t n = N; n > ROWS;) n = pgv_cdiv(n, ROWS), rows += n;   // (gn_param_grads_kernel's levels)
+    return 4 * rows * 2 * C;
+  }
   const int64_t stats = kind == 1 && !pl.fused ? 8 * N * G : 0;   // mean and rstd live here when the caller has no use for them
   return stats + (pl.fused ? 0 : 16 * N * G * pl.slices * pl.colblocks);
 }

@@ -863,6 +863,8 @@ class Fp8Linear(nn.Linear):
 
     def forward(self, x):
         x2 = x.reshape(-1, self.in_features)
+        if x2.shape[1] > 1 and (x2.stride(1) != 1 or x2.stride(0) < self.in_features):   # transposed or expanded
+            x2 = x2.contiguous()
         if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad or
                                         (self.bias is not None and self.bias.requires_grad)):
             y = Fp8LinearFn.apply(x2, self.weight, self.bias, self.grad_fmt)

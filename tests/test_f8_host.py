@@ -69,7 +69,7 @@ def test_group_norm_arguments(lib):
     refused(lib, f(act=4), b"activation")
     refused(lib, f(G=3), b"sizes")
     refused(lib, f(G=0), b"sizes")
-    refused(lib, f(N=70000), b"too large")
+    refused(lib, f(N=(1 << 24) + 1), b"too large")
     refused(lib, f(x=None), b"null")
     refused(lib, f(m=None), b"null")
     refused(lib, f(P=1 << 20), b"workspace", -3)

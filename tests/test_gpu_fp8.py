@@ -403,6 +403,14 @@ def test_module_trains_and_serves(ops):
         assert rel_l2(lin(x) - lin.bias, 2 * (plain - lin.bias)) < 1e-5
     lin.quantize_weight().train()
     assert lin._weight8 is None
+    lin.zero_grad()
+    wide = features(300, 6, torch.float32).cuda()                       # a transposed and an expanded input, as nn.Linear takes them
+    assert torch.equal(lin(wide.t()), lin(wide.t().contiguous()))
+    one = features(1, 300, torch.float32).cuda().requires_grad_(True)
+    lin(one.expand(5, 300)).sum().backward()
+    grad, one.grad = one.grad, None
+    lin(one.expand(5, 300).contiguous()).sum().backward()
+    assert torch.equal(grad, one.grad)
     frozen = layer.Fp8Linear(300, 130).cuda()
     frozen.weight.requires_grad_(False)
     frozen(x.detach().requires_grad_(True)).sum().backward()

@@ -91,7 +91,9 @@ SHAPES = [(1, 1, 32, 4), (1, 12, 2048, 32), (2, 391, 64, 8), (3, 17, 6, 3), (2, 
           (2, 100, 24, 3), (1, 1485, 96, 4), (2, 5000, 32, 8), (1, 3000, 20, 5), (1, 9, 4104, 3), (1, 600, 2600, 2), (1, 70, 2304, 96),
           (2, 700, 256, 32), (1, 4100, 512, 32), (1, 2, 16400, 2),
           # one wave per workgroup (many small slabs), the largest slabs in registers, and slices of 128 partial sums
-          (1100, 5, 32, 4), (300, 40, 128, 16), (2, 1485, 256, 16), (1, 1000, 64, 2), (2, 20000, 128, 4)]
+          (1100, 5, 32, 4), (300, 40, 128, 16), (2, 1485, 256, 16), (1, 1000, 64, 2), (2, 20000, 128, 4),
+          # many items (parameter gradients in two levels), one or two pixels (several groups per wave)
+          (2100, 1, 96, 3), (1030, 2, 20, 4), (70000, 1, 8, 2), (256, 1, 1024, 32)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
