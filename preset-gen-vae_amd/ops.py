@@ -950,8 +950,10 @@ def _f32_vector(who, name, t, n):
 
 def _f8_alloc(like, R, C, block, fmt):
     Kb = (C + 127) // 128
-    return Fp8Blocks(like.new_empty((R, Kb * 128), dtype=F8_FORMATS[fmt][1]),
-                     like.new_empty((Kb, R) if block == 'row' else ((R + 127) // 128, Kb), dtype=torch.float32), block, C)
+    dev, f32 = like.device, torch.float32
+    q = torch.empty(R, Kb * 128, dtype=F8_FORMATS[fmt][1], device=dev)
+    return Fp8Blocks(q, torch.empty(Kb, R, dtype=f32, device=dev) if block == 'row' else
+                     torch.empty((R + 127) // 128, Kb, dtype=f32, device=dev), block, C)
 
 
 def _f8_quantize(x, block, fmt, want, want_t, colsum=False):
@@ -964,7 +966,7 @@ def _f8_quantize(x, block, fmt, want, want_t, colsum=False):
     R, C = x.shape
     t = _f8_alloc(x, R, C, block, fmt) if want else None
     tt = _f8_alloc(x, C, R, block, fmt) if want_t else None
-    cs = x.new_empty(C, dtype=torch.float32) if colsum else None
+    cs = torch.empty(C, dtype=torch.float32, device=x.device) if colsum else None
     if R == 0 or C == 0:
         return t, tt, cs.zero_() if colsum else None
     ws = x.new_empty((R + 127) // 128 * C, dtype=torch.float32) if colsum else None
@@ -1024,7 +1026,7 @@ def _f8_out(who, like, M, N, dtype, out):
     if dtype not in _DT_CODE:
         raise ValueError(f"{who}: output type {dtype} is not float32, bfloat16 or float16")
     if out is None:
-        return like.new_empty((M, N), dtype=dtype)
+        return torch.empty(M, N, dtype=dtype, device=like.device)
     if out.device != like.device or out.dtype != dtype or tuple(out.shape) != (M, N) or not out.is_contiguous():
         raise ValueError(f"{who}: out must be a contiguous {dtype} [{M}, {N}] tensor on {like.device}")
     return out
@@ -1052,7 +1054,7 @@ def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16, out=None):
         return y.zero_() if bias is None else y.copy_(bias.expand(M, N))
     kind = F8_BLOCK_KINDS[b.block]
     nbytes = _f8_matmul_ws(M, N, K, kind)
-    ws = y.new_empty(nbytes // 4, dtype=torch.float32) if nbytes else None
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=y.device) if nbytes else None
     _lib.check(_lib.load().pgv_f8_matmul(M, N, K, a.q.data_ptr(), a.scale.data_ptr(), fmt, b.q.data_ptr(),
                                          b.scale.data_ptr(), kind, _p(bias), y.data_ptr(), _DT_CODE[y.dtype], _p(ws),
                                          nbytes, _raw_stream(y.get_device())), "pgv_f8_matmul")
@@ -1080,7 +1082,7 @@ def fp8_linear(x, w, bias=None, out_dtype=None, out=None):
         return y.zero_() if bias is None else y.copy_(bias.expand(M, N))
     kind = F8_BLOCK_KINDS[w.block]
     q_bytes, s_bytes, p_bytes = _f8_linear_ws(M, N, K, kind)      # one buffer: partial results, quantised rows, their scales
-    buf = x.new_empty(p_bytes + q_bytes + s_bytes, dtype=torch.uint8) if p_bytes + q_bytes else None   # (lives until the launches)
+    buf = torch.empty(p_bytes + q_bytes + s_bytes, dtype=torch.uint8, device=x.device) if p_bytes + q_bytes else None   # (lives until the launches)
     ws = None if buf is None else buf.data_ptr()
     _lib.check(_lib.load().pgv_f8_linear(x.data_ptr(), code, M, K, ld, w.q.data_ptr(), w.scale.data_ptr(), kind, N, _p(bias),
                                          ws + p_bytes if q_bytes else None, ws + p_bytes + q_bytes if q_bytes else None,
@@ -1164,11 +1166,12 @@ def group_norm_act_fwd(x, groups, weight=None, bias=None, eps=1e-5, act=PGV_ACT_
     if x.get_device() != _current_device():
         return _elsewhere(x, group_norm_act_fwd, x, groups, weight, bias, eps, act, slope)
     y = torch.empty_like(x)
-    mean, rstd = x.new_empty((N, groups), dtype=torch.float32), x.new_empty((N, groups), dtype=torch.float32)
+    dev, f32 = x.device, torch.float32
+    mean, rstd = torch.empty(N, groups, dtype=f32, device=dev), torch.empty(N, groups, dtype=f32, device=dev)
     if N == 0 or P == 0 or C == 0:
         return y, mean.zero_(), rstd.zero_()
     nbytes = _gn_ws(N, P, C, groups, code, _GN_FWD)
-    ws = x.new_empty(nbytes // 8, dtype=torch.float64) if nbytes else None
+    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=x.device) if nbytes else None
     _lib.check(_lib.load().pgv_group_norm_act_fwd(x.data_ptr(), code, N, P, C, groups, _p(weight), _p(bias), eps, act, slope,
                                                   y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _p(ws), nbytes, _raw_stream(x.get_device())),
                "pgv_group_norm_act_fwd")
@@ -1187,7 +1190,7 @@ def group_norm_act_fp8(x, groups, weight=None, bias=None, eps=1e-5, act=PGV_ACT_
     if x.numel() == 0:
         return t
     nbytes = _gn_ws(N, P, C, groups, code, _GN_F8)
-    ws = x.new_empty(nbytes // 8, dtype=torch.float64) if nbytes else None
+    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=x.device) if nbytes else None
     _lib.check(_lib.load().pgv_group_norm_act_f8(x.data_ptr(), code, N, P, C, groups, _p(weight), _p(bias), eps, act, slope,
                                                  F8_FORMATS[fmt][0], t.q.data_ptr(), t.scale.data_ptr(), _p(ws), nbytes,
                                                  _raw_stream(x.get_device())), "pgv_group_norm_act_f8")
@@ -1211,14 +1214,14 @@ def group_norm_act_bwd(gy, x, mean, rstd, groups, weight=None, bias=None, act=PG
     _f32_vector(who, "gbeta", gbeta, C)
     gx = torch.empty_like(x)
     if need_params:
-        ggamma = x.new_empty(C, dtype=torch.float32) if ggamma is None else ggamma
-        gbeta = x.new_empty(C, dtype=torch.float32) if gbeta is None else gbeta
+        ggamma = torch.empty(C, dtype=torch.float32, device=x.device) if ggamma is None else ggamma
+        gbeta = torch.empty(C, dtype=torch.float32, device=x.device) if gbeta is None else gbeta
     else:
         ggamma = gbeta = None
     if x.numel() == 0:
         return gx, ggamma.zero_() if need_params else None, gbeta.zero_() if need_params else None
     nbytes = _gn_ws(N, P, C, groups, code, _GN_BWD)
-    ws = x.new_empty(nbytes // 4, dtype=torch.float32)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device)
     _lib.check(_lib.load().pgv_group_norm_act_bwd(gy.data_ptr(), x.data_ptr(), code, N, P, C, groups, _p(weight), _p(bias),
                                                   mean.data_ptr(), rstd.data_ptr(), act, slope, gx.data_ptr(), _p(ggamma),
                                                   _p(gbeta), _p(ws), nbytes, _raw_stream(x.get_device())), "pgv_group_norm_act_bwd")
