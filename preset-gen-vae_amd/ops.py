@@ -1101,36 +1101,100 @@ class Fp8LinearSaved(NamedTuple):
     has_bias: bool
 
 
+def _align(n):
+    return (n + 255) // 256 * 256
+
+
+@functools.lru_cache(maxsize=4096)
+def _f8_train_ws(M, N, K):
+    """Byte offsets of the scratch of a forward (x: bytes, scales; w: bytes, scales; partial results) and of a backward pass (gy:
+    bytes, scales; its transpose: bytes, scales; column partials; partial results), and their ends."""
+    Kb, Nb, Mb = (K + 127) // 128, (N + 127) // 128, (M + 127) // 128
+
+    def offsets(*sizes):
+        out = [0]
+        for n in sizes:
+            out.append(out[-1] + _align(n))
+        return tuple(out)
+    fwd = offsets(M * Kb * 128, M * Kb * 4, N * Kb * 128, Nb * Kb * 4, _f8_matmul_ws(M, N, K, 1))
+    bwd = offsets(M * Nb * 128, M * Nb * 4, N * Mb * 128, N * Mb * 4, Mb * N * 4,
+                  max(_f8_matmul_ws(M, K, N, 1), _f8_matmul_ws(N, K, M, 0)))
+    return fwd, bwd
+
+
 def fp8_linear_fwd(x, w, bias=None):
     """nn.Linear of a training step: y = Q(x) Q(w)^T + bias in the type of x (x: 'row' blocks, w: 'tile' blocks, both e4m3), and
     the transposed operands its gradients contract over.  Returns (y, saved)."""
-    if w.dim() != 2 or x.dim() != 2 or x.shape[1] != w.shape[1]:
-        raise ValueError(f"fp8_linear_fwd: x {tuple(x.shape)} and w {tuple(w.shape)} do not match")
-    _same_device("fp8_linear_fwd", x, w, bias)
-    x8, xt8 = fp8_quantize_both(x, 'row')
-    w8, wt8 = fp8_quantize_both(w, 'tile')
-    y = fp8_matmul(x8, w8, bias, out_dtype=x.dtype)
-    return y, Fp8LinearSaved(xt8, wt8, x.dtype, w.dtype, bias is not None)
+    who = "fp8_linear_fwd"
+    xc, wc = _values(who, x), _values(who, w)
+    (M, K), N = x.shape, w.shape[0]
+    if w.shape[1] != K:
+        raise ValueError(f"{who}: x {tuple(x.shape)} and w {tuple(w.shape)} do not match")
+    if x.get_device() != _current_device():
+        return _elsewhere(x, fp8_linear_fwd, x, w, bias)
+    _same_device(who, x, w, bias)
+    if M == 0 or N == 0 or K == 0:      # (empty operands: their own checks and results)
+        x8, xt = fp8_quantize_both(x, 'row')
+        w8, wt = fp8_quantize_both(w, 'tile')
+        return fp8_matmul(x8, w8, bias, out_dtype=x.dtype), Fp8LinearSaved(xt, wt, x.dtype, w.dtype, bias is not None)
+    xl, wl = _row_stride(who, x), _row_stride(who, w)
+    _f32_vector(who, "bias", bias, N)
+    dev = x.device
+    y = torch.empty(M, N, dtype=x.dtype, device=dev)
+    xt, wt = _f8_alloc(x, K, M, 'row', 'e4m3'), _f8_alloc(x, K, N, 'tile', 'e4m3')
+    o = _f8_train_ws(M, N, K)[0]
+    buf = torch.empty(o[-1], dtype=torch.uint8, device=dev)
+    p, lib, stream = buf.data_ptr(), _lib.load(), _raw_stream(x.get_device())
+    _lib.check(lib.pgv_f8_quantize(x.data_ptr(), xc, M, K, xl, 0, 0, p, p + o[1], xt.q.data_ptr(), xt.scale.data_ptr(), None,
+                                   None, 0, stream), "pgv_f8_quantize")
+    _lib.check(lib.pgv_f8_quantize(w.data_ptr(), wc, N, K, wl, 1, 0, p + o[2], p + o[3], wt.q.data_ptr(), wt.scale.data_ptr(),
+                                   None, None, 0, stream), "pgv_f8_quantize")
+    _lib.check(lib.pgv_f8_matmul(M, N, K, p, p + o[1], 0, p + o[2], p + o[3], 1, _p(bias), y.data_ptr(), xc, p + o[4],
+                                 o[5] - o[4], stream), "pgv_f8_matmul")
+    return y, Fp8LinearSaved(xt, wt, x.dtype, w.dtype, bias is not None)
 
 
 def fp8_linear_bwd(gy, saved, grad_fmt='e4m3', need=(True, True, True), gw_out=None, gb_out=None):
     """Gradients of ``fp8_linear_fwd``: gx = Q(gy) Q(w) in the type of x, gw = Q(gy^T) Q(x^T)^T in the type of w, gb = the
     column sums of gy in float32 (None without a bias).  ``grad_fmt``: the 8-bit format of gy.  ``need``: which of (gx, gw,
     gb) are wanted; ``gw_out`` / ``gb_out``: buffers to write instead of new ones.  Returns (gx, gw, gb)."""
+    who = "fp8_linear_bwd"
     xt, wt, x_dtype, w_dtype, has_bias = saved
     (K, _), M, N = xt.q.shape, xt.cols, wt.cols
+    code = _values(who, gy)
     if tuple(gy.shape) != (M, N):
-        raise ValueError(f"fp8_linear_bwd: gy {tuple(gy.shape)}, expected {(M, N)}")
-    _same_device("fp8_linear_bwd", gy, xt.q)
-    need_gb = need[2] and has_bias
-    if not (need[0] or need[1] or need_gb):
+        raise ValueError(f"{who}: gy {tuple(gy.shape)}, expected {(M, N)}")
+    if grad_fmt not in F8_FORMATS:
+        raise ValueError(f"{who}: grad_fmt is 'e4m3' or 'e5m2', got {grad_fmt!r}")
+    if gy.get_device() != _current_device():
+        return _elsewhere(gy, fp8_linear_bwd, gy, saved, grad_fmt, need, gw_out, gb_out)
+    _same_device(who, gy, xt.q, wt.q, gw_out, gb_out)
+    need_gx, need_gw, need_gb = bool(need[0]), bool(need[1]), bool(need[2]) and has_bias
+    if not (need_gx or need_gw or need_gb):
         return None, None, None
-    g8, gt8, gb = _f8_quantize(gy, 'row', grad_fmt, need[0], need[1], colsum=need_gb)
-    if need_gb and gb_out is not None:
-        _f32_vector("fp8_linear_bwd", "gb_out", gb_out, N)
-        gb = gb_out.copy_(gb)
-    gx = fp8_matmul(g8, wt, out_dtype=x_dtype) if need[0] else None
-    gw = fp8_matmul(gt8, xt, out_dtype=w_dtype, out=gw_out) if need[1] else None
+    dev = gy.device
+    gx = torch.empty(M, K, dtype=x_dtype, device=dev) if need_gx else None
+    gw = _f8_out(who, gy, N, K, w_dtype, gw_out) if need_gw else None
+    if need_gb:
+        _f32_vector(who, "gb_out", gb_out, N)
+    gb = (torch.empty(N, dtype=torch.float32, device=dev) if gb_out is None else gb_out) if need_gb else None
+    if M == 0 or N == 0 or K == 0:      # sums over nothing
+        if need_gb and N:
+            gb.copy_(gy.sum(0, dtype=torch.float32)) if M else gb.zero_()
+        return gx.zero_() if need_gx else None, gw.zero_() if need_gw else None, gb
+    ld = _row_stride(who, gy)
+    o = _f8_train_ws(M, N, K)[1]
+    buf = torch.empty(o[-1], dtype=torch.uint8, device=dev)
+    p, lib, stream, fmt = buf.data_ptr(), _lib.load(), _raw_stream(gy.get_device()), F8_FORMATS[grad_fmt][0]
+    _lib.check(lib.pgv_f8_quantize(gy.data_ptr(), code, M, N, ld, 0, fmt, p if need_gx else None, p + o[1] if need_gx else None,
+                                   p + o[2] if need_gw else None, p + o[3] if need_gw else None, _p(gb), p + o[4], o[5] - o[4],
+                                   stream), "pgv_f8_quantize")
+    if need_gx:
+        _lib.check(lib.pgv_f8_matmul(M, K, N, p, p + o[1], fmt, wt.q.data_ptr(), wt.scale.data_ptr(), 1, None, gx.data_ptr(),
+                                     _DT_CODE[x_dtype], p + o[5], o[6] - o[5], stream), "pgv_f8_matmul")
+    if need_gw:
+        _lib.check(lib.pgv_f8_matmul(N, K, M, p + o[2], p + o[3], fmt, xt.q.data_ptr(), xt.scale.data_ptr(), 0, None,
+                                     gw.data_ptr(), _DT_CODE[w_dtype], p + o[5], o[6] - o[5], stream), "pgv_f8_matmul")
     return gx, gw, gb
 
 
