@@ -65,6 +65,9 @@ __device__ __forceinline__ f32x4 mfma128(const frag<F32>& b_rows, const frag<F32
   return d;
 }
 
+// first of n things that part k of `parts` takes (32-bit: n parts < 2^31 here, a 64-bit division is 100 instructions)
+__device__ __forceinline__ int split_at(int n, int k, int parts) { return parts == 1 ? k * n : (int)((unsigned)n * (unsigned)k / (unsigned)parts); }
+
 __device__ __forceinline__ i32x8 cat8(i32x4 lo, i32x4 hi) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
@@ -110,7 +113,7 @@ __global__ __launch_bounds__(64 * SW) void skinny_kernel(skinny_args p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16, split = blockIdx.z;
-  const int kb0 = (int)((int64_t)p.Kb * split / p.splits), kb1 = (int)((int64_t)p.Kb * (split + 1) / p.splits);
+  const int kb0 = split_at(p.Kb, split, p.splits), kb1 = split_at(p.Kb, split + 1, p.splits);
   const int64_t Kp = (int64_t)p.Kb * F8B;
   const uint8_t* bp = p.b + min(n0 + l16, p.N - 1) * Kp + g * 32;
   const float* sbp = p.sb + (int64_t)(n0 / F8B) * p.Kb;
@@ -285,7 +288,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) =
   tile_of(p, blockIdx.x, tm, tn);
   const int m0 = tm * BM, n0 = tn * BN;
   const int wm = (wave / NWN) * WM, wn = (wave % NWN) * WN;
-  const int kb0 = (int)((int64_t)p.Kb * split / p.splits), kb1 = (int)((int64_t)p.Kb * (split + 1) / p.splits);
+  const int kb0 = split_at(p.Kb, split, p.splits), kb1 = split_at(p.Kb, split + 1, p.splits);
   const uint32_t Kp = (uint32_t)p.Kb * F8B;
   const int rows_a = min(BM, p.M - m0), rows_b = min(BN, p.N - n0);
   const i32x4 rsrc_a = make_rsrc(p.a + (int64_t)m0 * Kp, rows_a * Kp), rsrc_b = make_rsrc(p.b + (int64_t)n0 * Kp, rows_b * Kp);

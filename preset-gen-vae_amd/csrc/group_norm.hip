@@ -34,6 +34,12 @@ struct gn_args {
   int lg;                        // log2 of the lanes that add up one group
 };
 
+// first pixel of a slice
+__device__ __forceinline__ int slice_at(const gn_args& p, int k) {
+  const int each = p.P / p.slices, more = p.P - each * p.slices;
+  return k * each + min(k, more);
+}
+
 // x / d for x d < 2^32 / d: the workgroup's own indices
 __device__ __forceinline__ int div_small(int x, int d, uint32_t magic) { return d == 1 ? x : (int)__umulhi((uint32_t)x, magic); }
 static inline uint32_t magic_of(int64_t d) { return d <= 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d); }
@@ -391,7 +397,7 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(gn_args p) {
   __shared__ sum2<double> val[256 * A];
   const int tid = threadIdx.x, item = blockIdx.x / p.slices, slice = blockIdx.x - item * p.slices, c0 = blockIdx.y * p.W;
   const place<SAME> q = my_place<SAME>(p, c0, 256);
-  const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
+  const int r0 = slice_at(p, slice), r1 = slice_at(p, slice + 1);
   const T* x = (const T*)p.x + (int64_t)item * p.P * p.C + q.c;
   sum2<double> s[A]{};
   auto take = [&](const raw8<T>& d) {
@@ -463,7 +469,7 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(gn_args p) {
     __syncthreads();
   }
   if (q.r >= q.rpp || (!Q && q.n == 0)) return;
-  const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
+  const int r0 = slice_at(p, slice), r1 = slice_at(p, slice + 1);
   const T* x = (const T*)p.x + (int64_t)item * p.P * p.C + q.c;
   chan<SAME> ch;
   if (p.parts) {
@@ -651,7 +657,7 @@ __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(gn_args p) {
   __shared__ float tot[4096];
   const int item = blockIdx.x / p.slices, slice = blockIdx.x - item * p.slices, c0 = blockIdx.y * p.W, width = min(p.W, p.C - c0);
   const place<SAME> q = my_place<SAME>(p, c0, 256);
-  const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
+  const int r0 = slice_at(p, slice), r1 = slice_at(p, slice + 1);
   const int64_t base = (int64_t)item * p.P * p.C + q.c;
   const T* x = (const T*)p.x + base;
   const T* gy = (const T*)p.gy + base;
@@ -731,7 +737,7 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(gn_args p, const floa
       [&](int) { return p.cg; }, [&](int g, const sum2<float>& v) { gs[0][g] = v.a * inv_n, gs[1][g] = v.b * inv_n; });
   __syncthreads();
   if (q.n == 0) return;
-  const int r0 = (int)((int64_t)p.P * slice / p.slices), r1 = (int)((int64_t)p.P * (slice + 1) / p.slices);
+  const int r0 = slice_at(p, slice), r1 = slice_at(p, slice + 1);
   const int64_t base = (int64_t)item * p.P * p.C + q.c;
   const T* x = (const T*)p.x + base;
   const T* gy = (const T*)p.gy + base;

@@ -341,6 +341,29 @@ def test_other_streams_and_captured_calls(ops):
                 assert torch.equal(a, b)
 
 
+def test_calls_from_two_threads(ops):
+    """Two threads, each on a stream of its own, with calls that need scratch: the results are those of calls one after the other."""
+    import threading
+    sizes = [(37, 300, 24576), (200, 72, 7000)]
+    data = [(features(M, K, torch.bfloat16).cuda(), ops.fp8_quantize(features(N, K, torch.float32, 5).cuda(), 'tile')) for M, N, K in sizes]
+    want = [ops.fp8_linear(x, w) for x, w in data]
+    got, streams = [[], []], [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+
+    def work(k):
+        with torch.cuda.stream(streams[k]):
+            for _ in range(30):
+                got[k].append(ops.fp8_linear(*data[k]))
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert len(got[k]) == 30 and all(torch.equal(y, want[k]) for y in got[k])
+
+
 def test_refusals(ops):
     x = features(8, 256, torch.float32).cuda()
     a, b = ops.fp8_quantize(x), ops.fp8_quantize(x, 'tile')

@@ -228,6 +228,39 @@ def test_block_of_the_three_operators(ops):
     assert all(torch.isfinite(p.grad).all() for p in [*norm.parameters(), *lin.parameters()])
 
 
+def test_captured_training_step(ops):
+    """Forward and backward of a small network of the modules in one graph, captured after a warm-up whose graphs are gone, replayed on
+    new values with eager steps between: every gradient equals the eager one."""
+    from preset_gen_vae_amd.model import layer
+    torch.manual_seed(5)
+    net = torch.nn.Sequential(layer.Fp8Linear(64, 128), layer.GroupNormAct(8, 128, activation=torch.nn.SiLU()),
+                              layer.Fp8Linear(128, 32, grad_fmt='e5m2')).cuda()
+    params = list(net.parameters())
+    x, gy = torch.randn(40, 64, device='cuda'), torch.randn(40, 32, device='cuda')
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            net.zero_grad(set_to_none=True)
+            net(x).backward(gy)
+    torch.cuda.current_stream().wait_stream(side)
+    net.zero_grad(set_to_none=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = net(x)
+        out.backward(gy)
+    captured = [p.grad for p in params]
+    out = out.detach()
+    for rep in range(3):
+        x.copy_(torch.randn(40, 64, generator=torch.Generator().manual_seed(rep)))
+        gy.copy_(torch.randn(40, 32, generator=torch.Generator().manual_seed(rep + 9)))
+        graph.replay()
+        y = net(x)
+        assert torch.equal(out, y)
+        for a, b in zip(captured, torch.autograd.grad(y, params, gy)):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("shape", [(2, 24, 9, 7), (3, 24), (2, 24, 11)])
 def test_module(ops, shape):
     from preset_gen_vae_amd.model import layer
