@@ -71,31 +71,36 @@ __device__ __forceinline__ void f8_scale(uint32_t bits, float& scale, float& inv
   inv = bad ? __uint_as_float(0x7fc00000u) : v;
 }
 
-// 8 consecutive values as floats; VEC: p is 16-byte aligned and all 8 lie inside, else only the first n are read (0 beyond)
-template <typename T>
+// a vector at an address that is a multiple of AL bytes only
+template <typename V, int AL>
+struct __attribute__((packed, aligned(AL), may_alias)) at_align {
+  V v;
+};
+
+// 8 consecutive values as floats, of which the first n exist (0 beyond).  VEC: p is 16-byte aligned; otherwise whole pieces are
+// the same loads at the alignment of a value.
+template <int AL, typename T>
 __device__ __forceinline__ void f8_load8_vec(const T* __restrict__ p, float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+    const at_align<f32x4, AL>* q = reinterpret_cast<const at_align<f32x4, AL>*>(p);
+    const f32x4 a = q[0].v, b = q[1].v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
   } else {
     typedef T t8 __attribute__((ext_vector_type(8)));
-    const t8 a = *reinterpret_cast<const t8*>(p);
+    const t8 a = reinterpret_cast<const at_align<t8, AL>*>(p)->v;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
   }
 }
-template <typename T>
-__device__ __forceinline__ void f8_load8_some(const T* __restrict__ p, int n, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.f;
-}
 template <bool VEC, typename T>
 __device__ __forceinline__ void f8_load8(const T* __restrict__ p, int n, float (&v)[8]) {
-  if (VEC && n >= 8)
-    f8_load8_vec(p, v);
-  else
-    f8_load8_some(p, n, v);
+  if (n >= 8) {
+    f8_load8_vec<VEC ? 16 : (int)sizeof(T)>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+  }
 }
 
 // one value of the output type, rounded once
