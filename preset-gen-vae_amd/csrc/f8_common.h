@@ -112,20 +112,20 @@ __device__ __forceinline__ void f8_store(void* out, int dt, int64_t i, float v) 
   else
     reinterpret_cast<_Float16*>(out)[i] = (_Float16)v;
 }
-// four neighbours; the address is a multiple of four values
+// four neighbours, at any multiple of a value
 __device__ __forceinline__ void f8_store4(void* out, int dt, int64_t i, f32x4 v) {
   if (dt == PGV_DT_F32) {
-    *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(out) + i) = v;
+    reinterpret_cast<at_align<f32x4, 4>*>(reinterpret_cast<float*>(out) + i)->v = v;
   } else if (dt == PGV_DT_BF16) {
     bf16x4 o;
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = (__bf16)v[j];
-    *reinterpret_cast<bf16x4*>(reinterpret_cast<__bf16*>(out) + i) = o;
+    reinterpret_cast<at_align<bf16x4, 2>*>(reinterpret_cast<__bf16*>(out) + i)->v = o;
   } else {
     f16x4 o;
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = (_Float16)v[j];
-    *reinterpret_cast<f16x4*>(reinterpret_cast<_Float16*>(out) + i) = o;
+    reinterpret_cast<at_align<f16x4, 2>*>(reinterpret_cast<_Float16*>(out) + i)->v = o;
   }
 }
 

@@ -376,7 +376,6 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) =
     }
     stage = stage + 1 == S ? 0 : stage + 1;
   }
-  const bool quad = (p.N & 3) == 0;
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
     const int n = n0 + wn + 16 * f + 4 * g;
@@ -392,7 +391,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) =
       void* out = p.splits > 1 ? (void*)(p.part + (int64_t)split * p.M * p.N) : p.out;
       const int dt = p.splits > 1 ? PGV_DT_F32 : p.out_dt;
       const f32x4 v = acc[f][i] + bv;
-      if (quad)
+      if (n + 4 <= p.N)
         f8_store4(out, dt, o, v);
       else
 #pragma unroll
