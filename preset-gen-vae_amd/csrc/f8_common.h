@@ -1,5 +1,6 @@
 // Shared helpers of the 8-bit (OCP e4m3 / e5m2) operand kernels: element types, conversion, the scale of a block.
 #pragma once
+#include <atomic>
 #include "pgv_common.h"
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -127,6 +128,21 @@ __device__ __forceinline__ void f8_store4(void* out, int dt, int64_t i, f32x4 v)
     for (int j = 0; j < 4; ++j) o[j] = (_Float16)v[j];
     reinterpret_cast<at_align<f16x4, 2>*>(reinterpret_cast<_Float16*>(out) + i)->v = o;
   }
+}
+
+// Raises a kernel's dynamic LDS limit, once per device (`done`: the kernel's own bit set of devices).
+static inline int f8_allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done, const char* who) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (e == hipSuccess && (done.load(std::memory_order_relaxed) & bit)) return PGV_OK;
+  if (e == hipSuccess) e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) {
+    pgv_set_error("%s: %d bytes of LDS refused: %s", who, bytes, hipGetErrorString(e));
+    return PGV_E_LAUNCH;
+  }
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return PGV_OK;
 }
 
 static inline int f8_dt_size(int dt) { return dt == PGV_DT_F32 ? 4 : 2; }

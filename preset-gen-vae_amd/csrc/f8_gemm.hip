@@ -271,8 +271,9 @@ __device__ __forceinline__ void tile_of(const tile_args& p, int wg, int& tm, int
 }
 
 // A stage in LDS is rows of 128 bytes (BM of a, BN of b), then 256 bytes of scales per wave.  The 16-byte piece c of row r sits
-// at piece c ^ (r & 7), so that the eight rows of a fragment read (same c) fall into different banks; LDS-DMA writes lane by
-// lane, so the permutation is applied to the address each lane fetches from.  S stages: S - 1 are in flight or complete while
+// at piece c ^ (r & 7) ^ (r >> 3 & 1), so that the 16 rows of a fragment read (same c) fall into different halves of different
+// banks (without the last term: 3.3 conflict cycles per read, the product 3 % slower); LDS-DMA writes lane by lane, so the
+// permutation is applied to the address each lane fetches from.  S stages: S - 1 are in flight or complete while
 // one is multiplied.  Every wave issues PW + 1 loads per stage: its pieces of 8 rows, and one of the scales.
 template <int BM, int BN, int WM, int WN, int S, bool BROW, int FA, bool F32>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) == 4 ? 2 : 1) void tile_kernel(tile_args p) {
@@ -407,11 +408,9 @@ int launch_tile(tile_args p, hipStream_t st) {
   p.tiles_n = (int)pgv_cdiv(p.N, BN);
   constexpr int threads = (BM / WM) * (BN / WN) * 64, lds = S * ((BM + BN) * F8B + threads * 4);
   auto k = tile_kernel<BM, BN, WM, WN, S, BROW, FA, F32>;
-  static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (once != hipSuccess) {
-    pgv_set_error("pgv_f8_matmul: %d bytes of LDS refused: %s", lds, hipGetErrorString(once));
-    return PGV_E_LAUNCH;
-  }
+  static std::atomic<uint64_t> done{0};
+  const int rc = f8_allow_lds((const void*)k, lds, done, "pgv_f8_matmul");
+  if (rc != PGV_OK) return rc;
   k<<<dim3((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits), threads, lds, st>>>(p);
   return PGV_OK;
 }

@@ -6,8 +6,9 @@
 // registers) and walks over pixels: a row of C channels is C / 8 threads and 16 or 32 bytes each.  Two schemes:
 //   fused     the pixels of one item and of a few whole groups fit in the registers of a workgroup: every value is read once,
 //             mean and variance are two passes over registers (the variance of x - mean: nothing cancels), one launch.
-//   two-pass  everything else: partial sums per slice of pixels, a finalising kernel, a second pass.  The slices' sums of x and
-//             x^2 are 64-bit ones: their difference is the variance, and it may be far smaller than either.
+//   two-pass  everything else: partial sums per slice of pixels, a second pass that reads the slices from their ends (what the
+//             first pass read last is still in the last-level cache).  The slices' sums of x and x^2 are 64-bit ones: their
+//             difference is the variance, and it may be far smaller than either.
 #include "f8_common.h"
 
 namespace {
@@ -41,7 +42,7 @@ __device__ __forceinline__ int slice_at(const gn_args& p, int k) {
   return k * each + min(k, more);
 }
 
-// x / d for x d < 2^32 / d: the workgroup's own indices
+// x / d for x d < 2^32: the workgroup's own indices
 __device__ __forceinline__ int div_small(int x, int d, uint32_t magic) { return d == 1 ? x : (int)__umulhi((uint32_t)x, magic); }
 static inline uint32_t magic_of(int64_t d) { return d <= 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d); }
 
@@ -921,11 +922,9 @@ int gn_forward(gn_args p, const gn_plan& pl, hipStream_t st) {
       } else if constexpr (SAME) {
         auto k = gn_fwd_fused_kernel<T, 1024, 16, 8, VEC, Q, FMT, SAME>;
         constexpr int lds = 8 * 1024 * 16;
-        static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        if (once != hipSuccess) {
-          pgv_set_error("pgv_group_norm_act: %d bytes of LDS refused: %s", lds, hipGetErrorString(once));
-          return PGV_E_LAUNCH;
-        }
+        static std::atomic<uint64_t> done{0};
+        const int rc = f8_allow_lds((const void*)k, lds, done, "pgv_group_norm_act");
+        if (rc != PGV_OK) return rc;
         k<<<grid, 1024, lds, st>>>(p);
       }
     }
@@ -946,11 +945,9 @@ template <typename T, int NT, int KV, bool VEC, bool SAME>
 int launch_bwd_fused(const gn_args& p, dim3 grid, hipStream_t st) {
   auto k = gn_bwd_fused_kernel<T, NT, KV, VEC, SAME>;
   constexpr int most = NT * 16 * (int)sizeof(float) + 2 * 8 * NT * (int)sizeof(float);   // W is at most 8 NT channels
-  static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, most);
-  if (once != hipSuccess) {
-    pgv_set_error("pgv_group_norm_act_bwd: %d bytes of LDS refused: %s", most, hipGetErrorString(once));
-    return PGV_E_LAUNCH;
-  }
+  static std::atomic<uint64_t> done{0};
+  const int rc = f8_allow_lds((const void*)k, most, done, "pgv_group_norm_act_bwd");
+  if (rc != PGV_OK) return rc;
   k<<<grid, NT, sizeof(float) * ((size_t)NT * 16 + 2 * (size_t)p.W), st>>>(p);
   return PGV_OK;
 }

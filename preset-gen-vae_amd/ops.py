@@ -1161,6 +1161,8 @@ def fp8_linear_bwd(gy, saved, grad_fmt='e4m3', need=(True, True, True), gw_out=N
     who = "fp8_linear_bwd"
     xt, wt, x_dtype, w_dtype, has_bias = saved
     (K, _), M, N = xt.q.shape, xt.cols, wt.cols
+    if wt.q.shape[0] != K or xt.block != 'row' or wt.block != 'tile':
+        raise ValueError(f"{who}: saved is not what fp8_linear_fwd returned")
     code = _values(who, gy)
     if tuple(gy.shape) != (M, N):
         raise ValueError(f"{who}: gy {tuple(gy.shape)}, expected {(M, N)}")
