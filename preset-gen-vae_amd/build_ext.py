@@ -9,12 +9,15 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libpgv_hip.so")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-Wno-unused-result"]
-# per-file extras: the FFT butterflies are complex arithmetic on register pairs - packing them into v_pk_* instructions
-# (SLP vectoriser) costs more register moves than it saves: 1560 -> 1376 instructions per frame pair without it
 # the 8-bit operand and group-norm kernels: without the packed fp32 instructions
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# per-file extras: the FFT butterflies are complex arithmetic on register pairs - packing them into v_pk_* instructions
+# (SLP vectoriser) costs more register moves than it saves: 1560 -> 1376 instructions per frame pair without it
 EXTRA = {"stft_mel.hip": ["-fno-slp-vectorize"], "f8_quant.hip": NO_PACKED_FP32, "f8_gemm.hip": NO_PACKED_FP32,
-         "group_norm.hip": NO_PACKED_FP32}
+         "group_norm.hip": NO_PACKED_FP32, "group_norm_f8.hip": NO_PACKED_FP32, "group_norm_bwd.hip": NO_PACKED_FP32}
+
+# the translation units that take longest to compile whatever their size
+LONG = ("group_norm_f8.hip", "group_norm_bwd.hip")
 
 
 def sources():
@@ -52,8 +55,8 @@ def build(force=False, verbose=True):
         if force or _stale(o, s, headers):
             cmd = [hipcc] + [f for f in FLAGS if f != "-shared"] + EXTRA.get(os.path.basename(s), []) + ["-c", s, "-o", o]
             todo.append((s, cmd))
-    # the long translation units first
-    todo.sort(key=lambda sc: -os.path.getsize(sc[0]))
+    # the long translation units first (most instantiations come from headers in two of them)
+    todo.sort(key=lambda sc: (os.path.basename(sc[0]) not in LONG, -os.path.getsize(sc[0])))
     jobs = max(1, int(os.environ.get("PGV_BUILD_JOBS", "8")))
     running = []
     while todo or running:
