@@ -4,6 +4,7 @@ import glob
 import os
 import subprocess
 import sys
+import time
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(HERE, "csrc")
@@ -63,11 +64,15 @@ def build(force=False, verbose=True):
         while todo and len(running) < jobs:
             s, cmd = todo.pop(0)
             running.append((s, subprocess.Popen(cmd)))
-        s, p = running.pop(0)
-        if p.wait() != 0:
-            for _, q in running:
-                q.kill()
-            raise RuntimeError(f"hipcc failed on {s}")
+        done = [sp for sp in running if sp[1].poll() is not None]   # (whichever ends first makes room for the next)
+        if not done:
+            time.sleep(0.05)
+        for s, p in done:
+            running.remove((s, p))
+            if p.returncode != 0:
+                for _, q in running:
+                    q.kill()
+                raise RuntimeError(f"hipcc failed on {s}")
     cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", OUT] + objs
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
